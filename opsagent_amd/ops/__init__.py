@@ -13,9 +13,10 @@ attention, activation, sampling) are the HIP kernels here.
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import os
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
@@ -28,8 +29,12 @@ __all__ = [
     "rope_apply_",
     "silu_mul",
     "kv_cache_write",
+    "KVPages",
+    "kv_cache_copy",
     "attention_prefill",
     "attention_decode_paged",
+    "shared_decode_plan",
+    "attention_decode_shared",
     "greedy_sample_masked",
     "rope_cos_sin",
 ]
@@ -1615,6 +1620,97 @@ def kv_cache_write(
     hip.check(rc, "oa_kv_write")
 
 
+class KVPages:
+    """The tensors of a paged cache, layer by layer, for :func:`kv_cache_copy`: looked over once.
+
+    ``layers``: (keys, values) of each layer, [pages, block, ...] each, either of them None where a
+    layer keeps none. Pages may lie any distance apart; what is in a page is dense. Values that
+    are a view of the key rows, and tensors that stand there twice, are copied once. The tensors
+    belong to the caller and are held here."""
+
+    def __init__(self, layers: Sequence[Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]]):
+        self.tensors: List[torch.Tensor] = []
+        for k, v in layers:
+            if k is None and v is None:
+                continue
+            if (k is not None and v is not None and v.dim() == k.dim() and v.dtype == k.dtype
+                    and v.data_ptr() == k.data_ptr() and v.stride() == k.stride()
+                    and v.shape[:-1] == k.shape[:-1] and v.shape[-1] <= k.shape[-1]):
+                v = None                       # the first channels of the key rows
+            self.tensors += [t for t in (k, v) if t is not None]
+        if not self.tensors:
+            raise ValueError("a cache without tensors has no pages")
+        first, seen = self.tensors[0], {}
+        for t in self.tensors:
+            if t.dim() < 2 or t.shape[:2] != first.shape[:2] or 0 in t.shape:
+                raise ValueError(f"cache tensors are [pages, block, ...] of one number of pages and "
+                                 f"tokens: got {tuple(t.shape)} beside {tuple(first.shape)}")
+            if t.device != first.device:
+                raise ValueError(f"cache tensors of {t.device} and {first.device}")
+            size = t[0].numel()
+            if not t[0].is_contiguous() or (t.shape[0] > 1 and t.stride(0) < size):
+                raise ValueError(f"a cache page has to be dense: strides {t.stride()}")
+            seen.setdefault((t.data_ptr(), t.shape, t.stride(), t.dtype), t)
+        self.tensors = list(seen.values())
+        self.num_pages, self.block_size = first.shape[:2]
+        self.device = first.device
+        # one launch for all tensors of one geometry: (bases, bytes of a page step, of a row)
+        self._launches = []
+        if first.is_cuda:
+            kinds = {}
+            for t in self.tensors:
+                row = t[0, 0].numel() * t.element_size()
+                step = t.stride(0) * t.element_size() if t.shape[0] > 1 else row * self.block_size
+                if (row | step | t.data_ptr()) % 16:
+                    raise ValueError("rows and pages of a cache on the GPU are multiples of 16 bytes")
+                kinds.setdefault((step, row), []).append(t.data_ptr())
+            for (step, row), at in kinds.items():
+                self._launches.append(((ctypes.c_uint64 * len(at))(*at), len(at), step, row))
+
+
+def kv_cache_copy(
+    pages: KVPages,
+    src: Sequence[int],
+    dst: Sequence[int],
+    tokens: Optional[Sequence[int]] = None,
+) -> None:
+    """Copies page src[i] to page dst[i] in every tensor of a cache, or its first tokens[i] rows:
+    forks of a sequence's last page, moves of a cache that is compacted. The lists lie on the host,
+    as the allocator's do. No page may be a target twice, or a source and a target: the copies
+    have no order."""
+    src, dst = list(src), list(dst)
+    n, block, last = len(src), pages.block_size, pages.num_pages
+    tokens = [block] * n if tokens is None else list(tokens)
+    if len(dst) != n or len(tokens) != n:
+        raise ValueError(f"{n} sources, {len(dst)} targets and {len(tokens)} numbers of tokens")
+    if n == 0:
+        return
+    if not all(isinstance(x, int) for part in (src, dst, tokens) for x in part):
+        raise TypeError("pages and tokens are ints on the host")
+    if min(src) < 0 or max(src) >= last or min(dst) < 0 or max(dst) >= last:
+        raise ValueError(f"page outside the cache of {last}")
+    if min(tokens) < 0 or max(tokens) > block:
+        raise ValueError(f"copies of a page of {block} tokens: got {min(tokens)} to {max(tokens)}")
+    targets = set(dst)
+    if len(targets) != n:
+        raise ValueError("a page is the target of two copies")
+    if not targets.isdisjoint(src):
+        raise ValueError("a page is the source of one copy and the target of another")
+    if not pages._launches:
+        for t in pages.tensors:
+            for i in range(n):
+                t[dst[i], : tokens[i]] = t[src[i], : tokens[i]]
+        return
+    lib, hip = _lib()
+    flat = (ctypes.c_int * (3 * n))()
+    flat[0::3], flat[1::3], flat[2::3] = src, dst, tokens
+    with torch.cuda.device(pages.device):
+        stream = hip.current_stream_ptr()
+        for bases, count, step, row in pages._launches:
+            hip.check(lib.oa_kv_pages_copy(stream, bases, count, step, row, block, last, flat, n),
+                      "oa_kv_pages_copy")
+
+
 def _prefill_splits(B: int, Hq: int, Hk: int, Sq: int, Skv: int) -> Tuple[int, bool]:
     """(key splits, merged form) of prefill attention; (1, False): not split.
 
@@ -1808,6 +1904,126 @@ def attention_decode_paged(
         1 if fused_combine else 0,
     )
     hip.check(rc, "oa_attention_decode")
+    return out
+
+
+class SharedPlan(NamedTuple):
+    """How a step's rows and pages are cut for attention_decode_shared: the same for all layers."""
+    ints: torch.Tensor
+    sizes: Tuple[int, ...]        # rows, heads, key heads, channels, table width, block size
+
+
+def _shared_sizes(B: int, Hq: int, Hk: int, D: int) -> Tuple[int, int]:
+    """Ints of a plan and slots of partial results."""
+    if not (1 <= B <= 2048 and Hk >= 1 and Hk <= Hq <= 4096 and Hq % Hk == 0 and D in (64, 128)):
+        raise ValueError(f"shared decode attention takes 1 to 2048 rows, heads in equal groups and "
+                         f"64 or 128 channels: got {B} rows, {Hq} heads on {Hk}, {D} channels")
+    ints, slots = ctypes.c_int(), ctypes.c_int()
+    lib, hip = _lib()
+    hip.check(lib.oa_shared_plan_size(B, Hq, Hk, D, ctypes.byref(ints), ctypes.byref(slots)),
+              "oa_shared_plan_size")
+    return ints.value, slots.value
+
+
+def _int_rows(device: torch.device, B: int, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name}: {B} int32 side by side on {device}, not {tuple(t.shape)} "
+                             f"{t.dtype} on {t.device}")
+
+
+def shared_decode_plan(
+    seq_lens: torch.Tensor,
+    leaders: torch.Tensor,
+    shared: torch.Tensor,
+    heads: Tuple[int, int],
+    head_dim: int,
+    width: int,
+    block_size: int,
+) -> Optional[SharedPlan]:
+    """The plan of attention_decode_shared for a step: made once, used by every layer. seq_lens,
+    leaders and shared [B] int32 as there; heads: (query, key) heads; width: columns of the block
+    table. It is made on the device, so a captured step that makes one follows its lengths and
+    leaders. None on the CPU, which needs none."""
+    if not _is_gpu(seq_lens):
+        return None
+    B, (Hq, Hk) = seq_lens.shape[0], heads
+    ints, _ = _shared_sizes(B, Hq, Hk, head_dim)
+    _int_rows(seq_lens.device, B, seq_lens=seq_lens, leaders=leaders, shared=shared)
+    if block_size < 1 or block_size & (block_size - 1) or not 1 <= width < 2 ** 31:
+        raise ValueError(f"a table of {width} pages of {block_size} tokens, not a power of 2")
+    lib, hip = _lib()
+    with torch.cuda.device(seq_lens.device):
+        plan = torch.empty(ints, dtype=torch.int32, device=seq_lens.device)
+        hip.check(lib.oa_shared_plan(
+            hip.current_stream_ptr(), seq_lens.data_ptr(), leaders.data_ptr(), shared.data_ptr(),
+            plan.data_ptr(), B, Hq, Hk, head_dim, width, block_size), "oa_shared_plan")
+    return SharedPlan(plan, (B, Hq, Hk, head_dim, width, block_size))
+
+
+def attention_decode_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    leaders: torch.Tensor,
+    shared: torch.Tensor,
+    scale: Optional[float] = None,
+    plan: Optional[SharedPlan] = None,
+) -> torch.Tensor:
+    """attention_decode_paged of a batch whose sequences begin with the same pages: those are read
+    once for all of them. q [B, Hq, D]; caches [pages, block, Hk, D] of q's type (bfloat16, float16;
+    64 or 128 channels); block_table [B, width] int32; out [B, Hq, D], zeros for rows without keys.
+
+    leaders, shared [B] int32: the first shared[b] pages of row b are those of row leaders[b]. A row
+    that shares nothing leads itself; so does one whose leader is no row that leads itself, or has
+    no keys. A group shares as many pages as all of its rows do, full ones only; sequences that grow
+    out of one prompt share more than that at times, which is read for each. ``plan``: of
+    shared_decode_plan for these lengths and leaders, made here where it is None. No gradients."""
+    if not _is_gpu(q):
+        return torch_ref.attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders,
+                                                 shared, scale)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or block_table.dim() != 2:
+        raise ValueError(f"q [B, Hq, D], caches [pages, block, Hk, D] and table [B, width]: got "
+                         f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}, "
+                         f"{tuple(block_table.shape)}")
+    B, Hq, D = q.shape
+    pages, block, Hk, _ = k_cache.shape
+    width = block_table.shape[1]
+    if k_cache.shape[3] != D or block_table.shape[0] != B or pages < 1 or width < 1:
+        raise ValueError(f"{B} rows of {D} channels, {k_cache.shape[3]} in the cache of {pages} pages, "
+                         f"a table of {tuple(block_table.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or not q.dtype == k_cache.dtype == v_cache.dtype:
+        raise ValueError(f"q and caches are of one 16-bit type: got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise RuntimeError("shared decode attention has no gradients")
+    if not q.device == k_cache.device == v_cache.device == block_table.device:
+        raise ValueError("q, caches and table are on one device")
+    if block_table.dtype != torch.int32 or (width > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table: rows of int32 side by side")
+    steps = (q.stride(0) if B > 1 else 0, q.stride(1) if Hq > 1 else 0,
+             *(t.stride(i) if t.shape[i] > 1 else 0 for t in (k_cache, v_cache) for i in range(3)))
+    if (q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1 or any(x % 8 for x in steps)
+            or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
+        raise ValueError("channels lie side by side, rows, pages and heads multiples of 16 bytes apart")
+    _int_rows(q.device, B, seq_lens=seq_lens, leaders=leaders, shared=shared)
+    _, slots = _shared_sizes(B, Hq, Hk, D)
+    if plan is None:
+        plan = shared_decode_plan(seq_lens, leaders, shared, (Hq, Hk), D, width, block)
+    elif plan.sizes != (B, Hq, Hk, D, width, block) or plan.ints.device != q.device:
+        raise ValueError(f"a plan of other sizes: {plan.sizes}, not {(B, Hq, Hk, D, width, block)}")
+    lib, hip = _lib()
+    with torch.cuda.device(q.device):
+        part = torch.empty(slots * Hq * (D + 2), dtype=torch.float32, device=q.device)
+        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+        hip.check(lib.oa_attention_decode_shared(
+            hip.current_stream_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            block_table.data_ptr(), plan.ints.data_ptr(), part.data_ptr(),
+            part.data_ptr() + slots * Hq * D * 4, out.data_ptr(),
+            (ctypes.c_int64 * 9)(*steps, block_table.stride(0) if B > 1 else 0),
+            B, Hq, Hk, D, pages, block, D ** -0.5 if scale is None else scale,
+            int(q.dtype == torch.float16)), "oa_attention_decode_shared")
     return out
 
 

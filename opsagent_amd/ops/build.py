@@ -23,6 +23,8 @@ SOURCES = [
     "sampling.hip",
     "attention_decode.hip",
     "attention_prefill.hip",
+    "attention_shared.hip",
+    "kv_pages.hip",
     "fp8_moe.hip",
     "moe_gemv.hip",
     "moe_grouped.hip",

@@ -114,6 +114,14 @@ def _declare(lib: ctypes.CDLL) -> None:
         i, i, i, i, i, i, i, f, i, i, i,
     ]
     lib.oa_attention_decode_rope.restype = i
+    lib.oa_shared_plan_size.argtypes = [i, i, i, i, p, p]
+    lib.oa_shared_plan_size.restype = i
+    lib.oa_shared_plan.argtypes = [p, p, p, p, p, i, i, i, i, i, i]
+    lib.oa_shared_plan.restype = i
+    lib.oa_attention_decode_shared.argtypes = [p] * 10 + [i] * 6 + [f, i]
+    lib.oa_attention_decode_shared.restype = i
+    lib.oa_kv_pages_copy.argtypes = [p, p, i, i64, i, i, i, p, i]
+    lib.oa_kv_pages_copy.restype = i
     lib.oa_quant_fp8.argtypes = [p, p, p, p, i, i]
     lib.oa_quant_fp8.restype = i
     lib.oa_silu_quant_fp8.argtypes = [p, p, p, p, i, i]

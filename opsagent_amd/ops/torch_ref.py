@@ -135,6 +135,47 @@ def attention_decode_paged(
     return torch.stack(outs).to(q.dtype)
 
 
+def attention_decode_shared(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    leaders: torch.Tensor,
+    shared: torch.Tensor,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """attention_decode_paged of rows whose first shared[b] pages are those of row leaders[b]
+    (a row that leads itself and has keys; any other row is its own): those pages are taken
+    from the leader's row of the table, as many as all of its rows share. Zeros for a row
+    without keys."""
+    B, Hq, D = q.shape
+    bs, Hk = k_cache.shape[1], k_cache.shape[2]
+    lens = [min(max(int(n), 0), block_table.shape[1] * bs) for n in seq_lens]
+    lead = [int(x) for x in leaders]
+    lead = [x if 0 <= x < B and lead[x] == x and lens[x] and lens[b] else b
+            for b, x in enumerate(lead)]
+    common = {}
+    for b, x in enumerate(lead):
+        pages = lens[b] // bs if x == b else min(max(int(shared[b]), 0), lens[b] // bs)
+        common.setdefault(x, []).append(pages)
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.zeros_like(q)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        row = block_table[b, : (n + bs - 1) // bs].long().clone()
+        group = common[lead[b]]
+        first = min(group) if len(group) > 1 else 0
+        row[:first] = block_table[lead[b], :first].long()
+        row = row.clamp(0, k_cache.shape[0] - 1)
+        k = k_cache[row].reshape(-1, Hk, D)[:n].float().repeat_interleave(Hq // Hk, dim=1)
+        v = v_cache[row].reshape(-1, Hk, D)[:n].float().repeat_interleave(Hq // Hk, dim=1)
+        p = torch.softmax(torch.einsum("hd,jhd->hj", q[b].float(), k) * scale, dim=-1)
+        out[b] = torch.einsum("hj,jhd->hd", p, v).to(q.dtype)
+    return out
+
+
 def kv_cache_write(
     k_cache: torch.Tensor,
     v_cache: torch.Tensor,
