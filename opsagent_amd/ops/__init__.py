@@ -1913,23 +1913,29 @@ class SharedPlan(NamedTuple):
     sizes: Tuple[int, ...]        # rows, heads, key heads, channels, table width, block size
 
 
+@functools.lru_cache(maxsize=1024)
 def _shared_sizes(B: int, Hq: int, Hk: int, D: int) -> Tuple[int, int]:
-    """Ints of a plan and slots of partial results."""
-    if not (1 <= B <= 2048 and Hk >= 1 and Hk <= Hq <= 4096 and Hq % Hk == 0 and D in (64, 128)):
-        raise ValueError(f"shared decode attention takes 1 to 2048 rows, heads in equal groups and "
-                         f"64 or 128 channels: got {B} rows, {Hq} heads on {Hk}, {D} channels")
+    """Ints of a plan, in whole 64 bytes, and slots of partial results."""
+    if not (1 <= B <= 2048 and 1 <= Hk <= Hq <= min(4096, 128 * Hk) and Hq % Hk == 0 and D in (64, 128)):
+        raise ValueError(f"shared decode attention takes 1 to 2048 rows, heads in equal groups of "
+                         f"up to 128 and 64 or 128 channels: got {B} rows, {Hq} heads on {Hk}, {D} channels")
     ints, slots = ctypes.c_int(), ctypes.c_int()
     lib, hip = _lib()
     hip.check(lib.oa_shared_plan_size(B, Hq, Hk, D, ctypes.byref(ints), ctypes.byref(slots)),
               "oa_shared_plan_size")
-    return ints.value, slots.value
+    return -(-ints.value // 16) * 16, slots.value
 
 
-def _int_rows(device: torch.device, B: int, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{name}: {B} int32 side by side on {device}, not {tuple(t.shape)} "
-                             f"{t.dtype} on {t.device}")
+@functools.lru_cache(maxsize=1024)
+def _shared_table(width: int, block: int) -> None:
+    if block < 1 or block & (block - 1) or not 1 <= width < 2 ** 31:
+        raise ValueError(f"a table of {width} pages of {block} tokens, which is no power of 2")
+
+
+def _int_rows(B: int, **rows: torch.Tensor) -> None:
+    for name, t in rows.items():
+        if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+            raise ValueError(f"{name}: {B} int32 side by side, not {tuple(t.shape)} {t.dtype}")
 
 
 def shared_decode_plan(
@@ -1948,10 +1954,11 @@ def shared_decode_plan(
     if not _is_gpu(seq_lens):
         return None
     B, (Hq, Hk) = seq_lens.shape[0], heads
+    _int_rows(B, seq_lens=seq_lens, leaders=leaders, shared=shared)
+    if not seq_lens.device == leaders.device == shared.device:
+        raise ValueError("seq_lens, leaders and shared are on one device")
     ints, _ = _shared_sizes(B, Hq, Hk, head_dim)
-    _int_rows(seq_lens.device, B, seq_lens=seq_lens, leaders=leaders, shared=shared)
-    if block_size < 1 or block_size & (block_size - 1) or not 1 <= width < 2 ** 31:
-        raise ValueError(f"a table of {width} pages of {block_size} tokens, not a power of 2")
+    _shared_table(width, block_size)
     lib, hip = _lib()
     with torch.cuda.device(seq_lens.device):
         plan = torch.empty(ints, dtype=torch.int32, device=seq_lens.device)
@@ -1959,6 +1966,33 @@ def shared_decode_plan(
             hip.current_stream_ptr(), seq_lens.data_ptr(), leaders.data_ptr(), shared.data_ptr(),
             plan.data_ptr(), B, Hq, Hk, head_dim, width, block_size), "oa_shared_plan")
     return SharedPlan(plan, (B, Hq, Hk, head_dim, width, block_size))
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_geometry(qs, q_steps, q_dtype, ks, k_steps, k_dtype, vs, v_steps, v_dtype, ts, t_steps, t_dtype):
+    """What attention_decode_shared takes of its tensors' sizes, strides and types, looked over once
+    for each: the sizes of the launch, ints of a plan, floats of partial results."""
+    if len(qs) != 3 or len(ks) != 4 or vs != ks or len(ts) != 2:
+        raise ValueError(f"q [B, Hq, D], caches [pages, block, Hk, D] and table [B, width]: got "
+                         f"{tuple(qs)}, {tuple(ks)}, {tuple(vs)}, {tuple(ts)}")
+    (B, Hq, D), (pages, block, Hk, _), width = qs, ks, ts[1]
+    if ks[3] != D or ts[0] != B or pages < 1 or width < 1:
+        raise ValueError(f"{B} rows of {D} channels, {ks[3]} in the cache of {pages} pages, a table of {tuple(ts)}")
+    if q_dtype not in (torch.bfloat16, torch.float16) or not q_dtype == k_dtype == v_dtype:
+        raise ValueError(f"q and caches are of one 16-bit type: got {q_dtype}, {k_dtype}, {v_dtype}")
+    if t_dtype != torch.int32 or (width > 1 and t_steps[1] != 1):
+        raise ValueError("block_table: rows of int32 side by side")
+    steps = (q_steps[0] if B > 1 else 0, q_steps[1] if Hq > 1 else 0,
+             *(s[i] if ks[i] > 1 else 0 for s in (k_steps, v_steps) for i in range(3)))
+    if q_steps[2] != 1 or k_steps[3] != 1 or v_steps[3] != 1 or any(x % 8 for x in steps):
+        raise ValueError("channels lie side by side, rows, pages and heads multiples of 16 bytes apart")
+    if max(steps[3], steps[6]) >= 2 ** 23:
+        raise ValueError("tokens of a page are less than 2^23 elements apart")
+    ints, slots = _shared_sizes(B, Hq, Hk, D)
+    _shared_table(width, block)
+    sizes = (ctypes.c_int64 * 17)(*steps, t_steps[0] if B > 1 else 0, B, Hq, Hk, D, width, pages, block,
+                                  q_dtype == torch.float16)
+    return sizes, ints, slots * Hq * (D + 2), (B, Hq, Hk, D, width, block)
 
 
 def attention_decode_shared(
@@ -1978,52 +2012,43 @@ def attention_decode_shared(
 
     leaders, shared [B] int32: the first shared[b] pages of row b are those of row leaders[b]. A row
     that shares nothing leads itself; so does one whose leader is no row that leads itself, or has
-    no keys. A group shares as many pages as all of its rows do, full ones only; sequences that grow
-    out of one prompt share more than that at times, which is read for each. ``plan``: of
-    shared_decode_plan for these lengths and leaders, made here where it is None. No gradients."""
+    no keys. A group shares as many pages as all of its rows do, full ones only; what some of its
+    rows share beyond that is read for each. ``plan``: of shared_decode_plan for these lengths and
+    leaders, made here where it is None. No gradients."""
     if not _is_gpu(q):
         return torch_ref.attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders,
                                                  shared, scale)
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or block_table.dim() != 2:
-        raise ValueError(f"q [B, Hq, D], caches [pages, block, Hk, D] and table [B, width]: got "
-                         f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}, "
-                         f"{tuple(block_table.shape)}")
-    B, Hq, D = q.shape
-    pages, block, Hk, _ = k_cache.shape
-    width = block_table.shape[1]
-    if k_cache.shape[3] != D or block_table.shape[0] != B or pages < 1 or width < 1:
-        raise ValueError(f"{B} rows of {D} channels, {k_cache.shape[3]} in the cache of {pages} pages, "
-                         f"a table of {tuple(block_table.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float16) or not q.dtype == k_cache.dtype == v_cache.dtype:
-        raise ValueError(f"q and caches are of one 16-bit type: got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    sizes, ints, floats, key = _shared_geometry(
+        q.shape, q.stride(), q.dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, v_cache.shape,
+        v_cache.stride(), v_cache.dtype, block_table.shape, block_table.stride(), block_table.dtype)
+    _int_rows(key[0], seq_lens=seq_lens, leaders=leaders, shared=shared)
+    device = q.get_device()
+    for t in (k_cache, v_cache, block_table, seq_lens, leaders, shared):
+        if t.get_device() != device:
+            raise ValueError(f"q, caches, table, lengths and leaders are on one device: got {t.device} "
+                             f"beside {q.device}")
+    at = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (at[0] | at[1] | at[2]) % 16:
+        raise ValueError("q and caches begin at multiples of 16 bytes")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("shared decode attention has no gradients")
-    if not q.device == k_cache.device == v_cache.device == block_table.device:
-        raise ValueError("q, caches and table are on one device")
-    if block_table.dtype != torch.int32 or (width > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table: rows of int32 side by side")
-    steps = (q.stride(0) if B > 1 else 0, q.stride(1) if Hq > 1 else 0,
-             *(t.stride(i) if t.shape[i] > 1 else 0 for t in (k_cache, v_cache) for i in range(3)))
-    if (q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1 or any(x % 8 for x in steps)
-            or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16):
-        raise ValueError("channels lie side by side, rows, pages and heads multiples of 16 bytes apart")
-    _int_rows(q.device, B, seq_lens=seq_lens, leaders=leaders, shared=shared)
-    _, slots = _shared_sizes(B, Hq, Hk, D)
-    if plan is None:
-        plan = shared_decode_plan(seq_lens, leaders, shared, (Hq, Hk), D, width, block)
-    elif plan.sizes != (B, Hq, Hk, D, width, block) or plan.ints.device != q.device:
-        raise ValueError(f"a plan of other sizes: {plan.sizes}, not {(B, Hq, Hk, D, width, block)}")
+    if plan is not None and (plan.sizes != key or plan.ints.get_device() != device):
+        raise ValueError(f"a plan of other sizes: {plan.sizes}, not {key}")
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders, shared,
+                                           scale, plan)
     lib, hip = _lib()
-    with torch.cuda.device(q.device):
-        part = torch.empty(slots * Hq * (D + 2), dtype=torch.float32, device=q.device)
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-        hip.check(lib.oa_attention_decode_shared(
-            hip.current_stream_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            block_table.data_ptr(), plan.ints.data_ptr(), part.data_ptr(),
-            part.data_ptr() + slots * Hq * D * 4, out.data_ptr(),
-            (ctypes.c_int64 * 9)(*steps, block_table.stride(0) if B > 1 else 0),
-            B, Hq, Hk, D, pages, block, D ** -0.5 if scale is None else scale,
-            int(q.dtype == torch.float16)), "oa_attention_decode_shared")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    room = torch.empty(floats + (ints if plan is None else 0), dtype=torch.float32, device=q.device)
+    start = room.data_ptr()
+    rc = lib.oa_attention_decode_shared(
+        hip.current_stream_ptr(), *at, block_table.data_ptr(),
+        *((seq_lens.data_ptr(), leaders.data_ptr(), shared.data_ptr(), start) if plan is None
+          else (None, None, None, plan.ints.data_ptr())),
+        start + 4 * ints if plan is None else start, out.data_ptr(), sizes,
+        key[3] ** -0.5 if scale is None else scale)
+    hip.check(rc, "oa_attention_decode_shared")
     return out
 
 

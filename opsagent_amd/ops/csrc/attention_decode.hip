@@ -96,17 +96,6 @@ __device__ __forceinline__ uint4 load_value(const uint32_t* p) {
     return __builtin_bit_cast(uint4, NT ? __builtin_nontemporal_load(at) : *at);
 }
 
-// inclusive sums over the wave's lanes, by row shifts and row broadcasts
-__device__ __forceinline__ int wave_sums(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
-}
-
 // Whether row b may be a copy of the first one. (All loads at once: each wait for memory would
 // add to every launch.)
 __device__ __forceinline__ bool maybe_copy(const int* slots, const int* seq_lens, int b, int copies) {

@@ -45,171 +45,225 @@ __device__ __forceinline__ uint32_t sh_pack(float lo, float hi) {
 }
 
 // ---- plan --------------------------------------------------------------------------------------
-// PLAN, in ints: units, slots (2, padded to 8) | first[B] | splits[B] | members[B], rows group after
-// group | units of 8: table row, first key, end, place of the group in members (-1: the table row
-// alone), first column, columns, split, 0. A column is a (member, head of the key head) pair.
+// PLAN, in ints: items (padded to 8) | first[B] | splits[B] | members[B], rows group after group |
+// units of 8: table row (-1: none), first key, end, place of the group's tile in members, members of
+// the tile (0: the table row alone), split, next unit of the item (-1: none), the table row's first slot.
 //
-// Keys of all jobs, a group's counted once for each tile of columns, are cut in about `target` equal
-// chunks; a job has as many of them as its keys need, of equal size, a multiple of 128.
-constexpr int PLAN_HEAD = 8, UNIT = 8;
+// A block takes items, each a chain of units; item i begins with unit i, and what follows in a chain
+// for row b is unit items + b. The items of a key head are to be of one size and as many as it has
+// blocks (`runs`). A group's pages are one item for each tile of columns and each of n equal chunks
+// of keys, tiles of a chunk side by side, so that they read the same keys at the same time. What lies
+// behind is put in a line, row after row, and cut in equal items at multiples of 128 keys of a row.
+// Sizes are in 64 keys, and a unit costs UNIT_COST of them beside its keys.
+constexpr int PLAN_HEAD = 8, UNIT = 8, UNIT_COST = 1;
 constexpr int PLAN_ROWS = 2048;
+constexpr int TILE = 128;                          // columns that a block takes
 
 struct PlanSizes {
-    int B, G, width, shift, tile, target, max_units, max_slots;
+    int B, G, width, shift, tile, runs, max_units, max_slots;    // tile: members of TILE columns
 };
 
-__device__ __forceinline__ int plan_chunk(int keys, int chunk) {
-    const int n = CEIL_DIV(keys, chunk);
-    return (CEIL_DIV(keys, n) + 127) & ~127;
+__host__ __device__ constexpr int plan_units(int B) { return (PLAN_HEAD + 3 * B + 3) & ~3; }   // 16-byte aligned
+__device__ __forceinline__ uint32_t cdiv(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+__device__ __forceinline__ uint32_t in_sizes(int keys) { return ((uint32_t)keys + 63) >> 6; }
+// chunks of a group's keys where an item has `run`, estimated; what a chunk has then; how many there are
+__device__ __forceinline__ int about_chunks(int keys, float per_run) { return (int)ceilf(in_sizes(keys) * per_run); }
+__device__ __forceinline__ int plan_chunk(int keys, float per_run) {
+    return ((int)cdiv(keys, max(about_chunks(keys, per_run), 1)) + 127) & ~127;
+}
+__device__ __forceinline__ int plan_chunks(int keys, float per_run) {
+    return keys > 0 ? (int)cdiv(keys, plan_chunk(keys, per_run)) : 0;
 }
 
-__global__ __launch_bounds__(1024) void shared_plan_kernel(const int* __restrict__ seq_lens,
-                                                           const int* __restrict__ leaders,
-                                                           const int* __restrict__ shared,
-                                                           int* __restrict__ plan, PlanSizes z) {
-    __shared__ int keys[PLAN_ROWS], lead[PLAN_ROWS], count[PLAN_ROWS], common[PLAN_ROWS], place[PLAN_ROWS];
-    __shared__ int total[16], chunk_all;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restrict__ seq_lens,
+                                                              const int* __restrict__ leaders,
+                                                              const int* __restrict__ shared,
+                                                              int* __restrict__ plan, PlanSizes z) {
+    constexpr int ROWS = THREADS == 1024 ? PLAN_ROWS : THREADS, NW = THREADS / WAVE, SIZES = 8;
+    // of a row: keys, leader, keys behind the shared ones, place in the line, chunks of the shared
+    // ones, first slot; of a leader: members, common keys, places in members and among the units
+    __shared__ int keys[ROWS], lead[ROWS], rests[ROWS], chunks[ROWS], slot_of[ROWS], count[ROWS], common[ROWS],
+        place[ROWS], unit_of[ROWS];
+    __shared__ uint32_t line[ROWS], total[NW], items_of[SIZES];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, B = z.B;
     const int most = (int)min((int64_t)z.width << z.shift, (int64_t)INT32_MAX - 4096);
-    for (int b = tid; b < B; b += 1024) {
+    auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_sums(v), WAVE - 1); };
+    for (int b = tid; b < B; b += THREADS) {
         keys[b] = min(max(seq_lens[b], 0), most);
         count[b] = 0;
         common[b] = INT32_MAX;
-        lead[b] = leaders[b];
+        place[b] = leaders[b];
     }
     __syncthreads();
     // a leader leads itself, and both have keys; any other row is its own
-    for (int b = tid; b < B; b += 1024) {
-        const int l = lead[b];
-        const bool led = l >= 0 && l < B && l != b && lead[l] == l && keys[b] > 0 && keys[l] > 0;
-        place[b] = led ? l : b;
+    for (int b = tid; b < B; b += THREADS) {
+        const int l = place[b];
+        const bool led = l >= 0 && l < B && l != b && place[l] == l && keys[b] > 0 && keys[l] > 0;
+        const int to = lead[b] = led ? l : b, pages = keys[b] >> z.shift;
+        atomicAdd(&count[to], 1);
+        atomicMin(&common[to], led ? min(max(shared[b], 0), pages) : pages);
     }
     __syncthreads();
-    for (int b = tid; b < B; b += 1024) lead[b] = place[b];
-    __syncthreads();
-    for (int b = tid; b < B; b += 1024) {
-        const int l = lead[b];
-        atomicAdd(&count[l], 1);
-        atomicMin(&common[l], l == b ? keys[b] >> z.shift : min(max(shared[b], 0), keys[b] >> z.shift));
-    }
-    __syncthreads();
-    // common: keys that a leader's group shares; and the keys of all jobs
-    const int tiles1 = CEIL_DIV(z.G, z.tile);
-    float all = 0.0f;
-    for (int b = tid; b < B; b += 1024) {
+    // common becomes the keys that a leader's group shares
+    int sum = 0;
+    for (int b = tid; b < B; b += THREADS)
         if (lead[b] == b) {
             common[b] = count[b] > 1 ? common[b] << z.shift : 0;
-            all += (float)common[b] * CEIL_DIV(count[b] * z.G, z.tile);
+            if (common[b]) sum += cdiv(count[b], z.tile) * (in_sizes(common[b]) + UNIT_COST);
         }
+    __syncthreads();
+    auto cost_of = [](int rest) { return rest > 0 ? in_sizes(rest) + UNIT_COST : 0u; };
+    for (int b = tid; b < B; b += THREADS) {
+        const int rest = rests[b] = keys[b] - common[lead[b]];
+        sum += cost_of(rest);
+    }
+    sum = wave_total(sum);
+    if (lane == 0) total[wave] = sum;
+    __syncthreads();
+    // the line
+    uint32_t all = 0, behind = 0;
+    for (int w = 0; w < NW; ++w) all += total[w];
+    for (int b0 = 0; b0 < B; b0 += WAVE) {
+        const int b = b0 + lane;
+        const uint32_t mine = b < B ? cost_of(rests[b]) : 0, sums = wave_sums(mine);
+        if (wave == 0 && b < B) line[b] = behind + sums - mine;
+        behind += __builtin_amdgcn_readlane(sums, WAVE - 1);
+    }
+    // the smallest size that needs no more items than there are blocks, of those from an equal share to
+    // one and a half times that
+    const uint32_t share = max(2u, cdiv(all, (uint32_t)z.runs));
+    auto size_of = [&](int i) { return share + share * i / (2 * SIZES); };
+    for (int i = wave; i < SIZES; i += NW) {
+        const uint32_t run = size_of(i);
+        const float per_run = 1.0f / run;
+        int n = 0;
+        for (int b = lane; b < B; b += WAVE)
+            if (common[b] > 0 && lead[b] == b) n += cdiv(count[b], z.tile) * about_chunks(common[b], per_run);
+        n = wave_total(n);
+        if (lane == 0) items_of[i] = n + cdiv(behind, run);
     }
     __syncthreads();
-    for (int b = tid; b < B; b += 1024) all += (float)(keys[b] - common[lead[b]]) * tiles1;
-    all = wave_reduce_sum(all);
-    if (lane == 0) total[wave] = __float_as_int(all);
-    __syncthreads();
-    if (tid == 0) {
-        float t = 0.0f;
-        for (int w = 0; w < 16; ++w) t += __int_as_float(total[w]);
-        const float c = fminf(ceilf(t / z.target), (float)(INT32_MAX / 2));
-        chunk_all = max(((int)c + 127) & ~127, 128);
-    }
-    __syncthreads();
-    const int chunk = chunk_all;
-    // places: the first wave adds up units, members and slots over the rows
+    int pick = 0;
+    while (pick < SIZES - 1 && items_of[pick] > (uint32_t)z.runs) ++pick;
+    const uint32_t run = size_of(pick);
+    const float per_run = 1.0f / run;
     int* const first = plan + PLAN_HEAD;
     int* const splits = first + B;
     int* const members = splits + B;
-    int* const units = members + B;
-    __shared__ int unit_of[PLAN_ROWS], member_of[PLAN_ROWS];
+    int* const units = plan + plan_units(B);
+    // places of the groups' units and members
+    int ahead = 0, at = 0;
+    for (int b0 = 0; b0 < B; b0 += WAVE) {
+        const int b = b0 + lane;
+        int nu = 0, nm = 0;
+        if (b < B && lead[b] == b) {
+            const int n = plan_chunks(common[b], per_run);
+            if (n) {
+                nm = count[b];
+                nu = (int)cdiv(nm, z.tile) * n;
+            }
+            if (wave == 0) chunks[b] = n;
+        }
+        const int iu = wave_sums(nu), im = wave_sums(nm);
+        if (wave == 0 && b < B) {
+            unit_of[b] = ahead + iu - nu;
+            place[b] = at + im - nm;
+        }
+        ahead += __builtin_amdgcn_readlane(iu, WAVE - 1);
+        at += __builtin_amdgcn_readlane(im, WAVE - 1);
+    }
+    // items of the line, and how much of it each has
+    int lines = (int)cdiv(behind, run);
+    if (behind > 0 && ahead + lines < z.runs) lines = (int)min((uint32_t)(z.runs - ahead), max(behind / 2, 1u));
+    const uint32_t step = lines > 0 ? max(2u, cdiv(behind, lines)) : 1;
+    if (lines > 0) lines = (int)cdiv(behind, step);
+    const int items = ahead + lines;
+    // Item i of the line begins where i * step falls, rounded to 128 keys of the row there: a row at
+    // `line` is cut by the items that fall from line + 1 to the middle of its last 128 keys, and those
+    // from there to the next row's first place begin with that row.
+    auto cuts_from = [&](int b) { return (int)cdiv(line[b] + 1, step); };
+    auto cuts_to = [&](int b) { return (int)cdiv(line[b] + 2 * ((uint32_t)(rests[b] + 127) >> 7) - 1, step); };
+    auto cut = [&](int b, int i) { return (int)((i * step - line[b] + 1) >> 1 << 7); };
+    __syncthreads();
     if (wave == 0) {
-        int u = 0, m = 0, s = 0;
+        int s = 0;
         for (int b0 = 0; b0 < B; b0 += WAVE) {
             const int b = b0 + lane;
-            int nu = 0, nm = 0, ns = 0;
+            int ns = 0;
             if (b < B) {
-                const int l = lead[b], p = common[l], rest = keys[b] - p;
-                if (p > 0) ns = CEIL_DIV(p, plan_chunk(p, chunk));
-                if (l == b && p > 0) {
-                    nm = count[b];
-                    nu = ns * CEIL_DIV(count[b] * z.G, z.tile);
-                }
-                if (rest > 0) {
-                    const int c = CEIL_DIV(rest, plan_chunk(rest, chunk));
-                    ns += c;
-                    nu += c * tiles1;
-                }
+                ns = chunks[lead[b]];
+                if (rests[b] > 0) ns += 1 + cuts_to(b) - cuts_from(b);
             }
-            int iu = nu, im = nm, is = ns;
-#pragma unroll
-            for (int d = 1; d < WAVE; d <<= 1) {
-                const int a = __shfl_up(iu, d, WAVE), e = __shfl_up(im, d, WAVE), f = __shfl_up(is, d, WAVE);
-                if (lane >= d) {
-                    iu += a;
-                    im += e;
-                    is += f;
-                }
-            }
+            const int is = wave_sums(ns);
             if (b < B) {
-                unit_of[b] = u + iu - nu;
-                member_of[b] = m + im - nm;
-                first[b] = s + is - ns;
+                first[b] = slot_of[b] = s + is - ns;
                 splits[b] = ns;
             }
-            u += __shfl(iu, WAVE - 1, WAVE);
-            m += __shfl(im, WAVE - 1, WAVE);
-            s += __shfl(is, WAVE - 1, WAVE);
+            s += __builtin_amdgcn_readlane(is, WAVE - 1);
         }
-        if (lane == 0) {
-            plan[0] = min(u, z.max_units);
-            plan[1] = s;
-        }
+        if (lane == 0) plan[0] = min(items, z.max_units);
     }
     __syncthreads();
-    // a wave a row: members of its group in order, and its units
-    for (int b = wave; b < B; b += 16) {
-        const int l = lead[b], p = common[l], rest = keys[b] - p;
-        int u = unit_of[b], done = 0;
-        if (l == b && p > 0) {
-            for (int b0 = 0, m = member_of[b]; b0 < B; b0 += WAVE) {
-                const bool mine = b0 + lane < B && lead[b0 + lane] == b;
-                const uint64_t all_mine = __ballot(mine);
-                if (mine) members[m + __builtin_popcountll(all_mine & ((1ull << lane) - 1))] = b0 + lane;
-                m += __builtin_popcountll(all_mine);
-            }
-            const int c = plan_chunk(p, chunk), columns = count[b] * z.G;
-            const int n = CEIL_DIV(p, c), tiles = CEIL_DIV(columns, z.tile);
-            for (int i = lane; i < n * tiles; i += WAVE) {
-                if (u + i >= z.max_units) break;
-                int* d = units + (size_t)(u + i) * UNIT;
-                const int part = i / tiles, col = i % tiles * z.tile;
-                d[0] = b;
-                d[1] = part * c;
-                d[2] = min(part * c + c, p);
-                d[3] = member_of[b];
-                d[4] = col;
-                d[5] = min(z.tile, columns - col);
-                d[6] = part;
-                d[7] = 0;
-            }
-            u += n * tiles;
+    auto write = [&](int u, int row, int k0, int k1, int place, int n, int split, int next) {
+        if (u >= z.max_units) return;
+        int4* d = reinterpret_cast<int4*>(units) + 2 * (size_t)u;
+        d[0] = int4{row, k0, k1, place};
+        d[1] = int4{n, split, next < z.max_units ? next : -1, row >= 0 ? slot_of[row] : 0};
+    };
+    // a wave a group: its members in order, and its units
+    for (int b = wave; b < B; b += NW) {
+        const int p = common[b];
+        if (lead[b] != b || p <= 0) continue;
+        for (int b0 = 0, m = place[b]; b0 < B; b0 += WAVE) {
+            const bool mine = b0 + lane < B && lead[b0 + lane] == b;
+            const uint64_t all_mine = __ballot(mine);
+            if (mine) members[m + __builtin_popcountll(all_mine & ((1ull << lane) - 1))] = b0 + lane;
+            m += __builtin_popcountll(all_mine);
         }
-        if (p > 0) done = CEIL_DIV(p, plan_chunk(p, chunk));
-        if (rest > 0) {
-            const int c = plan_chunk(rest, chunk), n = CEIL_DIV(rest, c);
-            for (int i = lane; i < n * tiles1; i += WAVE) {
-                if (u + i >= z.max_units) break;
-                int* d = units + (size_t)(u + i) * UNIT;
-                const int part = i / tiles1, col = i % tiles1 * z.tile;
-                d[0] = b;
-                d[1] = p + part * c;
-                d[2] = min(p + part * c + c, keys[b]);
-                d[3] = -1;
-                d[4] = col;
-                d[5] = min(z.tile, z.G - col);
-                d[6] = done + part;
-                d[7] = 0;
-            }
+        const int c = plan_chunk(p, per_run), tiles = (int)cdiv(count[b], z.tile);
+        for (int i = lane; i < chunks[b] * tiles; i += WAVE) {
+            const int part = i / tiles, from = i % tiles * z.tile;
+            write(unit_of[b] + i, b, part * c, min(part * c + c, p), place[b] + from, min(z.tile, count[b] - from), part, -1);
         }
+    }
+    // the unit behind a row's last one in its item: the next row's first, unless that begins an item
+    auto after = [&](int b) {
+        while (++b < B && rests[b] <= 0) {}
+        return b;
+    };
+    auto link = [&](int b) {
+        const int next = after(b);
+        return next < B && cuts_from(next) == cuts_to(b) ? items + next : -1;
+    };
+    // a thread a row: its first unit, and the items that have none, of those that fall between the
+    // last row's last cut and this one, or behind the last row
+    for (int b = tid; b < B; b += THREADS) {
+        const int rest = rests[b];
+        if (rest <= 0) continue;
+        int before = b - 1;
+        while (before >= 0 && rests[before] <= 0) --before;
+        const int from = before >= 0 ? cuts_to(before) : 0, own = cuts_from(b), to = cuts_to(b);
+        for (int i = from; i < own - 1; ++i) write(ahead + i, -1, 0, 0, 0, 0, 0, -1);
+        if (after(b) == B)
+            for (int i = to; i < lines; ++i) write(ahead + i, -1, 0, 0, 0, 0, 0, -1);
+        const int p = keys[b] - rest, n = chunks[lead[b]];
+        write(from < own ? ahead + own - 1 : items + b, b, p, p + (own < to ? cut(b, own) : rest), 0, 0, n,
+              own < to ? -1 : link(b));
+    }
+    // a thread an item of the line: the unit that it begins with, where that is not a row's first
+    for (int i = tid; i < lines; i += THREADS) {
+        int b = 0, end = B;                      // the last row that begins at or before it
+        while (end - b > 1) {
+            const int mid = (b + end) / 2;
+            if (line[mid] <= (uint32_t)i * step) b = mid;
+            else end = mid;
+        }
+        const int own = cuts_from(b), to = cuts_to(b);
+        if (rests[b] <= 0 || i < own || i >= to) continue;
+        const int p = keys[b] - rests[b];
+        write(ahead + i, b, p + cut(b, i), p + (i + 1 < to ? cut(b, i + 1) : rests[b]), 0, 0, chunks[lead[b]] + 1 + i - own,
+              i + 1 < to ? -1 : link(b));
     }
 }
 
@@ -225,172 +279,336 @@ struct SharedArgs {
     float scale;                                                                 // times log2(e)
 };
 
-// A block takes the chunk of a unit for one key head, its four waves 32 keys in turn. Keys are the
-// rows of the first product (S^T = K Q^T: a lane has the scores of one column, four keys of every
-// sixteen), and the contraction of the second (O^T = V^T P^T) takes a lane's own weights as they
-// are, keys 4g..+3 and 16 + 4g..+3 for lane group g; the transposing LDS read gives the values in
-// the same order. MT: tiles of 16 columns.
-template <bool F16, int D, int MT>
-__device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __restrict__ unit, int h, char* lds) {
-    constexpr int NS = D / 32, ND = D / 16, ROW = D * 2, PIECES = ROW / 16;
-    const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, g = lane >> 4;
+struct SharedUnit {
+    int row, begin, end, place, group, split, slot, columns;
+};
+
+// Four waves take a unit's chunk for one key head. A wave has up to 32 columns (MT tiles of 16), so
+// KG groups of waves share the keys out, 32 in turn, and the 4 / KG waves of a group the columns:
+//     columns     up to 32     64     128
+//     KG                 4      2       1
+// Keys are the rows of the first product (S^T = K Q^T: a lane has the scores of one column, four keys
+// of every sixteen), and the contraction of the second (O^T = V^T P^T) takes a lane's own weights as
+// they are, keys 4g..+3 and 16 + 4g..+3 for lane group g; the transposing LDS read gives the values
+// in the same order.
+//
+// Keys and values come by 16-byte transfers into LDS, 16 KiB a step of 32 keys and 128 channels, and
+// a group has a ring of 4 / KG steps. A group of one wave asks for the next keys while it works on
+// the values and for the next values behind that, with no barrier; the others have one a step. Two
+// blocks fit a CU (LDS), so that one's ends and barriers are the other's work.
+//
+// 16-byte pieces of key rows and 32-byte pieces of value rows change places with the key, so that
+// neither the reads of key rows nor the transposing ones meet in a bank; a transfer writes LDS in
+// lane order, so its source address carries the change.
+constexpr int IDS = 1024;                          // pages of a unit that lie in LDS at a time
+
+template <int N>
+__device__ __forceinline__ void wait_transfers() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+__device__ __forceinline__ const char* same_in_wave(const char* p) {
+    const uint64_t v = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (const char*)((uint64_t)hi << 32 | lo);
+}
+
+// maximum over the four lane groups
+__device__ __forceinline__ float over_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <bool F16, int D, int MT, int KG>
+__device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUnit& unit, int h, char* lds) {
+    constexpr int NS = D / 32, ND = D / 16, ROW = D * 2, CPR = ROW / 16;
+    constexpr int CG = 4 / KG, KEYS = KG == 1 ? 64 : 32, STAGES = KG == 4 ? 1 : 2;
+    constexpr int PLANE = KEYS * ROW, STAGE = 2 * PLANE, NJ = KEYS / 16;
+    constexpr int RPP = 1024 / ROW, PCS = 32 / RPP;          // rows of a transfer, transfers of 32 rows
+    constexpr int COLS = CG * 32;
+    int lane = threadIdx.x & (WAVE - 1);
+    asm volatile("" : "+v"(lane));           // places in LDS are worked out here, not kept from unit to unit
+    const int col = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int row0 = unit[0], k0 = unit[1], k1 = unit[2], group = unit[3], c0 = unit[4], columns = unit[5];
-    const int* const table = a.block_table + row0 * a.table_row;
-    const int* const members = a.plan + PLAN_HEAD + 2 * a.B;
-    const int G = a.G;
+    const int kg = wave / CG, cg = wave % CG;
+    const int row0 = unit.row, begin = unit.begin, end = unit.end, columns = unit.columns;
+    const int* const members = unit.group ? a.plan + PLAN_HEAD + 2 * a.B + unit.place : nullptr;
+    const int G = a.G, mask = (1 << a.shift) - 1;
+    constexpr int RING = 4 * 32 * D * 4, MERGE = 4 * 32 * (D + 4 + 2) * 4;
+    int* const ids = reinterpret_cast<int*>(lds + (RING > MERGE ? RING : MERGE));
+    int* const slots = ids + IDS;                            // of the tile's members
+    const int* const first = a.plan + PLAN_HEAD;
+    if (members)
+        for (int i = threadIdx.x; i < unit.group; i += 256) slots[i] = first[members[i]];
+    char* const ring = lds + kg * (RING / KG);
+    const uint32_t ring_at = (uint32_t)(uintptr_t)ring;
 
     uint4 qf[MT][NS];
+    const bool busy = cg * 32 < columns;                     // the wave has columns
+    // signs of q so that larger products are larger weights; no q at all where the scale is 0
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep_q = a.scale == 0.0f ? 0u : ~0u;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        const int c = m * 16 + col;
+        const int c = cg * 32 + m * 16 + col;
         const bool in = c < columns;
-        const int cc = in ? c0 + c : c0;
-        const int b = group < 0 ? row0 : members[group + cc / G];
+        const int cc = in ? c : 0;
+        const int b = members ? members[cc / G] : row0;
         const char* at = a.q + b * a.q_row + (h * G + cc % G) * a.q_head + g * 16;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const uint4 w = *reinterpret_cast<const uint4*>(at + s * 64);
-            qf[m][s] = in ? w : uint4{0, 0, 0, 0};
+            qf[m][s] = in ? uint4{(w.x ^ flip) & keep_q, (w.y ^ flip) & keep_q, (w.z ^ flip) & keep_q, (w.w ^ flip) & keep_q}
+                          : uint4{0, 0, 0, 0};
         }
     }
     sh_f4 o[MT][ND];
-    float mx[MT], sum[MT];
+    // sums of weights come from the matrix cores too, as the product with values of 1: of the rounded
+    // weights, which the outputs are made of
+    sh_f4 sum[MT];
+    float mx[MT];
+    const uint32_t one = F16 ? 0x3c003c00u : 0x3f803f80u;
+    const uint4 ones = {one, one, one, one};
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         mx[m] = -INFINITY;
-        sum[m] = 0.0f;
+        sum[m] = sh_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[m][d] = sh_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const char* const kb = a.kc + h * a.k_head;
     const char* const vb = a.vc + h * a.v_head;
-    const int mask = (1 << a.shift) - 1;
-    // keys past the chunk's end are its last one: what it has is read, nothing that no row owns
-    auto page_of = [&](int key) { return min((uint32_t)table[key >> a.shift], (uint32_t)(a.pages - 1)); };
-    char* const vt = lds + wave * (32 * ROW);
-    // 32-byte pieces of a value row change places with the key, so that the 16 keys that one
-    // transposing read gathers lie in all banks
-    auto swz = [](int key) { return D == 128 ? key & 7 : (key >> 1) & 3; };
+    auto swz_k = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    auto swz_v = [](int r) { return D == 128 ? r & 7 : (r >> 1) & 3; };
 
-    for (int at = k0 + wave * 32; at < k1; at += 128) {
-        uint4 kf[2][NS];
+    // the unit's keys in spans whose pages lie in LDS; what a table should not hold reads the last page
+    const int span = (int)min((int64_t)(IDS - 16) << a.shift & ~(int64_t)127, (int64_t)INT32_MAX / 2);
+    int k0 = begin, k1 = begin + min(span, end - begin), page0 = k0 >> a.shift;
+    auto place_pages = [&]() {
+        const int* const table = a.block_table + row0 * a.table_row;
+        page0 = k0 >> a.shift;
+        for (int i = threadIdx.x; i <= ((k1 - 1) >> a.shift) - page0; i += 256)
+            ids[i] = (int)min((uint32_t)table[page0 + i], (uint32_t)(a.pages - 1));
+    };
+    place_pages();
+    // 32 rows of keys or values from `key` on. What lies past the chunk is its last key, so that
+    // nothing that no row owns is read.
+    const int r_lane = lane / CPR, pc = lane % CPR;
+    auto load_rows = [&](bool values, int key, uint32_t to) {
+        key = __builtin_amdgcn_readfirstlane(key);
+        to = __builtin_amdgcn_readfirstlane(to);
+        const char* const base = values ? vb : kb;
+        const int64_t step = values ? a.v_page : a.k_page;
+        const int token = (int)(values ? a.v_token : a.k_token);
+        const int last = k1 - 1 - key;
+        auto place_of = [&](int p, int& at) {                // in the row; and the row
+            const int r = p * RPP + r_lane;
+            at = min(r, last);
+            return (values ? (((pc >> 1) ^ swz_v(r)) << 1 | (pc & 1)) : pc ^ swz_k(r)) * 16;
+        };
+        if (a.shift >= 5) {                                  // rows of one page
+            const int page = __builtin_amdgcn_readfirstlane(ids[(key >> a.shift) - page0]);
+            const char* const rows = same_in_wave(base + page * step + (int64_t)(key & mask) * token);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int key = min(at + j * 16 + col, k1 - 1);
-            const char* p = kb + page_of(key) * a.k_page + (key & mask) * a.k_token + g * 16;
+            for (int p = 0; p < 32 / RPP; ++p) {
+                int at;
+                const int place = place_of(p, at);
+                lds_transfer16(to + p * 1024, __umul24(at, token) + place, rows);
+            }
+        } else {
 #pragma unroll
-            for (int s = 0; s < NS; ++s) kf[j][s] = *reinterpret_cast<const uint4*>(p + s * 64);
+            for (int p = 0; p < 32 / RPP; ++p) {
+                int at;
+                const int place = place_of(p, at), kk = key + at;
+                lds_transfer16(to + p * 1024, base + ids[(kk >> a.shift) - page0] * step + (int64_t)(kk & mask) * token + place);
+            }
         }
-        uint4 vf[PIECES / 2];
-#pragma unroll
-        for (int t = 0; t < PIECES / 2; ++t) {
-            const int piece = t * WAVE + lane, r = piece / PIECES, u = piece % PIECES;
-            const int key = min(at + r, k1 - 1);
-            const int src = ((u >> 1) ^ swz(r)) * 32 + (u & 1) * 16;
-            vf[t] = *reinterpret_cast<const uint4*>(vb + page_of(key) * a.v_page + (key & mask) * a.v_token + src);
-        }
-#pragma unroll
-        for (int t = 0; t < PIECES / 2; ++t) *reinterpret_cast<uint4*>(vt + (t * WAVE + lane) * 16) = vf[t];
+    };
 
-        uint4 pf[MT];
+    // a step's keys from LDS: scores, weights, and their product with the values. The first values are
+    // read ahead of the weights.
+    constexpr int EARLY = ND / 2;
+    uint4 pf[MT][NJ / 2];
+    sh_f4 sc[MT][NJ];
+    auto products = [&](const char* kt) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            float w[8];
+        for (int j = 0; j < NJ; ++j) {
+            uint4 kf[NS];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                sh_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int s = 0; s < NS; ++s)
+                kf[s] = *reinterpret_cast<const uint4*>(kt + (j * 16 + col) * ROW + ((s * 4 + g) ^ swz_k(j * 16 + col)) * 16);
 #pragma unroll
-                for (int s = 0; s < NS; ++s) acc = sh_product<F16>(kf[j][s], qf[m][s], acc);
+            for (int m = 0; m < MT; ++m) {
+                sc[m][j] = sh_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) sc[m][j] = sh_product<F16>(kf[s], qf[m][s], sc[m][j]);
+            }
+        }
+    };
+    auto weights = [&](int key) {
+        if (key + KEYS > k1) {
+            asm volatile("" : : : "memory");                 // a branch: every other step goes without
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    w[j * 4 + r] = at + j * 16 + g * 4 + r < k1 ? acc[r] * a.scale : -INFINITY;
-            }
-            float top = w[0];
+                    if (key + j * 16 + g * 4 + r >= k1)
 #pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, w[i]);
-            top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-            top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+                        for (int m = 0; m < MT; ++m) sc[m][j][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            float top = sc[m][0][0];
+#pragma unroll
+            for (int i = 1; i < NJ * 4; ++i) top = fmaxf(top, sc[m][i >> 2][i & 3]);
+            top = over_groups(top);
             if (__any(top > mx[m])) {
                 const float now = fmaxf(top, mx[m]);
-                const float old = mx[m] == now ? 1.0f : exp2f(mx[m] - now);
+                const float keep = mx[m] == now ? 1.0f : __builtin_amdgcn_exp2f((mx[m] - now) * scale);
                 mx[m] = now;
-                sum[m] *= old;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[m][r] *= keep;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[m][d][r] *= old;
+                    for (int r = 0; r < 4; ++r) o[m][d][r] *= keep;
             }
-            const float base = mx[m] == -INFINITY ? 0.0f : mx[m];
+            const float base = mx[m] == -INFINITY ? 0.0f : mx[m] * scale;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = exp2f(w[i] - base);
-                sum[m] += w[i];
+            for (int i = 0; i < NJ * 4; ++i)
+                sc[m][i >> 2][i & 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][i >> 2][i & 3], scale, -base));
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2)
+                pf[m][j / 2] = uint4{sh_pack<F16>(sc[m][j][0], sc[m][j][1]), sh_pack<F16>(sc[m][j][2], sc[m][j][3]),
+                                     sh_pack<F16>(sc[m][j + 1][0], sc[m][j + 1][1]),
+                                     sh_pack<F16>(sc[m][j + 1][2], sc[m][j + 1][3])};
+        }
+    };
+    auto value = [&](const char* vt, int half, int d) {
+        union {
+            struct { sh_s4 lo, hi; } p;
+            uint4 u;
+        } v;
+        const int r = half * 32 + g * 4 + (col >> 2);
+        const char* lo = vt + r * ROW + (d ^ swz_v(r)) * 32 + (col & 3) * 8;
+        const char* hi = vt + (r + 16) * ROW + (d ^ swz_v(r + 16)) * 32 + (col & 3) * 8;
+        v.p.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)lo);
+        v.p.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)hi);
+        return v.u;
+    };
+    auto add_values = [&](const char* vt, const uint4* early) {
+#pragma unroll
+        for (int half = 0; half < NJ / 2; ++half) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) sum[m] = sh_product<F16>(ones, pf[m][half], sum[m]);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const uint4 v = early && half == 0 && d < EARLY ? early[d] : value(vt, half, d);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) o[m][d] = sh_product<F16>(v, pf[m][half], o[m][d]);
             }
-            pf[m] = uint4{sh_pack<F16>(w[0], w[1]), sh_pack<F16>(w[2], w[3]), sh_pack<F16>(w[4], w[5]),
-                          sh_pack<F16>(w[6], w[7])};
         }
-        // the wave's own values: written above, read below
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            union {
-                struct { sh_s4 lo, hi; } p;
-                uint4 u;
-            } v;
-            const int r = g * 4 + (col >> 2);
-            const char* lo = vt + r * ROW + (d ^ swz(r)) * 32 + (col & 3) * 8;
-            const char* hi = vt + (r + 16) * ROW + (d ^ swz(r + 16)) * 32 + (col & 3) * 8;
-            v.p.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)lo);
-            v.p.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)hi);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) o[m][d] = sh_product<F16>(v.u, pf[m], o[m][d]);
+    };
+
+    for (;;) {
+    __syncthreads();                                         // ids
+    if constexpr (KG == 4) {
+        int key = k0 + kg * 32;
+        if (key < k1) {
+            load_rows(false, key, ring_at);
+            load_rows(true, key, ring_at + PLANE);
         }
-        __builtin_amdgcn_wave_barrier();
+        for (; key < k1; key += 128) {
+            wait_transfers<PCS>();
+            products(ring);
+            wait_reads();
+            const bool more = key + 128 < k1;
+            if (more) load_rows(false, key + 128, ring_at);
+            weights(key);
+            if (more) wait_transfers<PCS>();
+            else wait_transfers<0>();
+            add_values(ring + PLANE, nullptr);
+            wait_reads();
+            if (more) load_rows(true, key + 128, ring_at + PLANE);
+        }
+    } else {
+        // a wave brings 32 rows of a step: the first waves keys, the others values
+        static_assert(CG * 32 == 2 * KEYS, "as many waves as there are 32 rows");
+        // steps of the block, and of this group
+        const int steps = CEIL_DIV(k1 - k0, KEYS * KG), mine = CEIL_DIV(k1 - k0 - kg * KEYS, KEYS * KG);
+        auto key_of = [&](int i) { return k0 + (i * KG + kg) * KEYS; };
+        auto ask = [&](int i) {
+            const int half = cg % (KEYS / 32) * 32, key = key_of(i) + half;
+            const bool values = cg >= KEYS / 32;
+            // a step's second half may lie past the chunk: any rows of it do
+            if (i < mine)
+                load_rows(values, key < k1 ? key : key - half, ring_at + i % STAGES * STAGE + (values ? PLANE : 0) + half * ROW);
+        };
+        ask(0);
+        for (int i = 0; i < steps; ++i) {
+            // this step has come, and nobody is at the one before
+            wait_transfers<0>();
+            wait_reads();
+            asm volatile("s_barrier" : : : "memory");
+            ask(i + 1);
+            const char* const at = ring + i % STAGES * STAGE;
+            if (busy && i < mine) {
+                products(at);
+                uint4 early[EARLY];
+#pragma unroll
+                for (int d = 0; d < EARLY; ++d) early[d] = value(at + PLANE, 0, d);
+                weights(key_of(i));
+                add_values(at + PLANE, early);
+            }
+        }
+    }
+    if (k1 >= end) break;
+    __syncthreads();                                         // all have read the span's pages
+    k0 = k1;
+    k1 = k0 + min(span, end - k0);
+    place_pages();
     }
 
-    // the waves' sums: a common maximum of each column, then each wave's share of the channels
+    // a common maximum of the groups' sums of each column, in units of the weights' exponent
     __syncthreads();
     constexpr int PITCH = D + 4;
-    float* const merge = reinterpret_cast<float*>(lds);                       // [4][MT * 16][PITCH]
-    float* const stats = merge + 4 * MT * 16 * PITCH;                         // [4][MT * 16][2]
+    float* const merge = reinterpret_cast<float*>(lds);                       // [KG][COLS][PITCH]
+    float* const stats = merge + KG * COLS * PITCH;                           // [KG][COLS][2]
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        sum[m] += __shfl_xor(sum[m], 16, WAVE);
-        sum[m] += __shfl_xor(sum[m], 32, WAVE);
-        if (g == 0) {
-            float* s = stats + (wave * MT * 16 + m * 16 + col) * 2;
-            s[0] = mx[m];
-            s[1] = sum[m];
-        }
+        const int c = cg * 32 + m * 16 + col;
+        if (c >= columns) continue;
+        if (g == 0)
+            *reinterpret_cast<float2*>(stats + (kg * COLS + c) * 2) =
+                float2{mx[m] == -INFINITY ? -INFINITY : mx[m] * scale, sum[m][0]};
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-            *reinterpret_cast<sh_f4*>(merge + (wave * MT * 16 + m * 16 + col) * PITCH + d * 16 + g * 4) = o[m][d];
+            *reinterpret_cast<sh_f4*>(merge + (kg * COLS + c) * PITCH + d * 16 + g * 4) = o[m][d];
     }
     __syncthreads();
-    const int* const first = a.plan + PLAN_HEAD;
     for (int i = threadIdx.x; i < columns * (D / 4); i += 256) {
         const int c = i / (D / 4), ch = i % (D / 4) * 4;
-        float ms[4], top = -INFINITY;
+        float2 st[KG];
+        float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            ms[w] = stats[(w * MT * 16 + c) * 2];
-            top = fmaxf(top, ms[w]);
+        for (int w = 0; w < KG; ++w) {
+            st[w] = *reinterpret_cast<const float2*>(stats + (w * COLS + c) * 2);
+            top = fmaxf(top, st[w].x);
         }
-        const float base = top == -INFINITY ? 0.0f : top;
         float l = 0.0f;
         sh_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = ms[w] == base ? 1.0f : exp2f(ms[w] - base);
-            l += stats[(w * MT * 16 + c) * 2 + 1] * f;
-            acc += *reinterpret_cast<const sh_f4*>(merge + (w * MT * 16 + c) * PITCH + ch) * f;
+        for (int w = 0; w < KG; ++w) {
+            const float f = st[w].x == top ? 1.0f : __builtin_amdgcn_exp2f(st[w].x - top);
+            l += st[w].y * f;
+            acc += *reinterpret_cast<const sh_f4*>(merge + (w * COLS + c) * PITCH + ch) * f;
         }
-        const int cc = c0 + c;
-        const int b = group < 0 ? row0 : members[group + cc / G];
-        const int slot = first[b] + unit[6];
+        const int slot = (members ? slots[c / G] : unit.slot) + unit.split;
         if (slot >= a.slots) continue;
-        const size_t to = (size_t)slot * a.Hq + h * G + cc % G;
+        const size_t to = (size_t)slot * a.Hq + h * G + c % G;
         *reinterpret_cast<sh_f4*>(a.o_part + to * D + ch) = acc;
         if (ch == 0) *reinterpret_cast<float2*>(a.ml_part + to * 2) = float2{top, l};
     }
@@ -398,44 +616,111 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const int* __re
 
 // Grid: units times key heads, the heads of a unit side by side: with eight of them a key head is on
 // one die, whose L2 then has a chunk for all tiles of columns.
-template <bool F16, int D, int MT>
-__global__ __launch_bounds__(256) void shared_attn_kernel(SharedArgs a) {
-    constexpr int RING = 4 * 32 * D * 2, MERGE = 4 * MT * 16 * (D + 4 + 2) * 4;
-    __shared__ __attribute__((aligned(16))) char lds[RING > MERGE ? RING : MERGE];
-    const int u = blockIdx.x / a.Hk, h = blockIdx.x % a.Hk;
-    if (u >= a.plan[0]) return;
-    const int* unit = a.plan + PLAN_HEAD + 3 * a.B + (size_t)u * UNIT;
-    if (MT > 1 && unit[5] <= 16) shared_unit<F16, D, 1>(a, unit, h, lds);
-    else shared_unit<F16, D, MT>(a, unit, h, lds);
+template <bool F16, int D>
+__global__ __launch_bounds__(256, 2) void shared_attn_kernel(SharedArgs a) {
+    constexpr int RING = 4 * 32 * D * 4, MERGE = 4 * 32 * (D + 4 + 2) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[(RING > MERGE ? RING : MERGE) + (IDS + TILE) * 4];
+    const int h = blockIdx.x % a.Hk;
+    const int* const units = a.plan + plan_units(a.B);
+    // the number of items and the first one's record in one wait: there is room for `runs` of them
+    const int4* const mine = reinterpret_cast<const int4*>(units) + 2 * (size_t)(blockIdx.x / a.Hk);
+    const int count = a.plan[0];
+    int4 x = mine[0], y = mine[1];
+    const int items = __builtin_amdgcn_readfirstlane(count);
+    for (int i = blockIdx.x / a.Hk; i < items; i += gridDim.x / a.Hk)
+        for (int u = i; u >= 0;) {
+            if (u != (int)(blockIdx.x / a.Hk)) {
+                const int4* const at = reinterpret_cast<const int4*>(units) + 2 * (size_t)u;
+                x = at[0];
+                y = at[1];
+            }
+            auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+            SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(x.w), same(y.x), same(y.y), same(y.w), 0};
+            const int columns = unit.columns = max(unit.group, 1) * a.G;
+            u = same(y.z);
+            if ((uint32_t)unit.row >= (uint32_t)a.B) continue;   // an item without units
+            if (columns <= 16) shared_unit<F16, D, 1, 4>(a, unit, h, lds);
+            else if (columns <= 32) shared_unit<F16, D, 2, 4>(a, unit, h, lds);
+            else if (columns <= 64) shared_unit<F16, D, 2, 2>(a, unit, h, lds);
+            else shared_unit<F16, D, 2, 1>(a, unit, h, lds);
+            __syncthreads();                                 // LDS is the next unit's
+        }
 }
 
-// A wave a (row, head): the slots' sums with their common maximum.
-template <bool F16, int D>
+// PER waves take a (row, head): the slots' sums with their common maximum. Weights of up to 64 slots
+// are worked out by a lane each; sums are read eight at a time.
+template <bool F16, int D, int PER>
 __global__ __launch_bounds__(256) void shared_combine_kernel(const float* __restrict__ o_part,
                                                              const float* __restrict__ ml_part,
                                                              const int* __restrict__ plan, char* __restrict__ out,
                                                              int B, int Hq, int slots) {
-    const int pair = blockIdx.x * 4 + threadIdx.x / WAVE, lane = threadIdx.x & (WAVE - 1);
-    if (pair >= B * Hq) return;
+    constexpr int CH = D / WAVE;
+    __shared__ float red[4][D + 2];
+    const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int pair = blockIdx.x * (4 / PER) + wave / PER, part = wave % PER;
+    if (pair >= B * Hq) return;                              // with PER > 1 all of a block or none
     const int b = pair / Hq, h = pair % Hq;
     const int s0 = plan[PLAN_HEAD + b];
     const int n = min(plan[PLAN_HEAD + B + b], slots - s0);
-    float top = -INFINITY;
-    for (int s = lane; s < n; s += WAVE) top = fmaxf(top, ml_part[((size_t)(s0 + s) * Hq + h) * 2]);
-    top = wave_reduce_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    constexpr int CH = D / WAVE;
-    float acc[CH], total = 0.0f;
+    const float2* const ml = reinterpret_cast<const float2*>(ml_part) + (size_t)s0 * Hq + h;
+    const float* const o = o_part + ((size_t)s0 * Hq + h) * D + lane * CH;
+    float top = -INFINITY, acc[CH], total = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) acc[c] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-        const size_t at = (size_t)(s0 + s) * Hq + h;
-        const float2 ml = *reinterpret_cast<const float2*>(ml_part + at * 2);
-        const float f = ml.x == base ? 1.0f : exp2f(ml.x - base);
-        total += ml.y * f;
+    const int parts = n > part ? CEIL_DIV(n - part, PER) : 0;         // slots part, part + PER, ...
+    for (int b0 = 0; b0 < parts; b0 += WAVE) {
+        const int here = min(parts - b0, WAVE);
+        const float2 mine = lane < here ? ml[(size_t)((b0 + lane) * PER + part) * Hq] : float2{-INFINITY, 0.0f};
+        const float now = fmaxf(top, wave_reduce_max(mine.x));
+        const float base = now == -INFINITY ? 0.0f : now;
+        const float keep = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - base);
+        const float f = mine.x == base ? 1.0f : __builtin_amdgcn_exp2f(mine.x - base);
+        top = now;
+        total = total * keep + wave_reduce_sum(mine.y * f);
 #pragma unroll
-        for (int c = 0; c < CH; ++c) acc[c] += o_part[at * D + lane * CH + c] * f;
+        for (int c = 0; c < CH; ++c) acc[c] *= keep;
+        for (int s = 0; s < here; s += 8) {
+            float v[8][CH];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float* const at = o + (size_t)((b0 + min(s + i, here - 1)) * PER + part) * Hq * D;
+                if constexpr (CH == 2) {
+                    const float2 w = *reinterpret_cast<const float2*>(at);
+                    v[i][0] = w.x;
+                    v[i][1] = w.y;
+                } else {
+                    v[i][0] = *at;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = __shfl(f, min(s + i, here - 1), WAVE);
+                if (s + i < here)
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) acc[c] += v[i][c] * w;
+            }
+        }
+    }
+    if constexpr (PER > 1) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) red[wave][lane * CH + c] = acc[c];
+        if (lane == 0) {
+            red[wave][D] = top;
+            red[wave][D + 1] = total;
+        }
+        __syncthreads();
+        if (part) return;
+        for (int w = 0; w < PER; ++w) top = fmaxf(top, red[w][D]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        total = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) acc[c] = 0.0f;
+        for (int w = 0; w < PER; ++w) {
+            const float f = red[w][D] == base ? 1.0f : __builtin_amdgcn_exp2f(red[w][D] - base);
+            total += red[w][D + 1] * f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) acc[c] += red[w][lane * CH + c] * f;
+        }
     }
     const float r = total == 0.0f ? 1.0f : total;
     if constexpr (CH == 2)
@@ -445,28 +730,24 @@ __global__ __launch_bounds__(256) void shared_combine_kernel(const float* __rest
 }
 
 // ---- entries -----------------------------------------------------------------------------------
-// Columns that a block takes, and chunks that the keys of a key head are cut in: about two blocks a CU.
-static int shared_tiles(int B, int G) { return (int64_t)B * G <= 16 ? 1 : (int64_t)B * G <= 32 ? 2 : 4; }
-static int shared_target(int Hk) { return max(1, 512 / Hk); }
-
 static bool shared_sizes(int B, int Hq, int Hk, int D) {
-    return B >= 1 && B <= PLAN_ROWS && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Hq <= 4096 && (D == 64 || D == 128);
+    return B >= 1 && B <= PLAN_ROWS && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Hq <= 4096 && Hq / Hk <= TILE && (D == 64 || D == 128);
 }
 
-// Units: chunks of `target` and one more for each job (rows, and a group's tiles of columns, of which
-// there are at the most B * G / tile and one more for each of B / 2 groups). Slots: a chunk of a
-// group's tile leaves tile / G of them, and every row has one more of each kind.
+// Blocks of a key head: two a CU. Units: items, of which there are at the most `runs` and one for each
+// tile of a group (B / tile and one more for each of B / 2 groups) beside as many of the line, and one
+// more a row. Slots: what an item of a tile leaves is a slot for each of its members, of which there
+// are `tile` or B, and a row has one more of each kind than equal shares would make.
 static PlanSizes plan_sizes(int B, int Hq, int Hk, int width, int shift) {
     PlanSizes z;
     z.B = B;
     z.G = Hq / Hk;
     z.width = width;
     z.shift = shift;
-    z.tile = 16 * shared_tiles(B, z.G);
-    z.target = shared_target(Hk);
-    const int64_t tiles1 = CEIL_DIV(z.G, z.tile);
-    z.max_units = (int)(z.target + (int64_t)B * z.G / z.tile + B / 2 + z.target + B * tiles1 + 8);
-    z.max_slots = (int)((int64_t)z.tile * z.target / z.G + z.target + 2 * (int64_t)B + 8);
+    z.tile = max(1, TILE / z.G);
+    z.runs = max(1, 512 / Hk);
+    z.max_units = 2 * z.runs + B / z.tile + B / 2 + B + 16;
+    z.max_slots = (min(z.tile, B) + 1) * z.runs + 4 * B + 16;
     return z;
 }
 
@@ -474,73 +755,102 @@ static PlanSizes plan_sizes(int B, int Hq, int Hk, int width, int shift) {
 extern "C" int oa_shared_plan_size(int B, int Hq, int Hk, int D, int* ints, int* slots) {
     if (!shared_sizes(B, Hq, Hk, D)) return -100;
     const PlanSizes z = plan_sizes(B, Hq, Hk, 1, 0);
-    *ints = PLAN_HEAD + 3 * B + z.max_units * UNIT;
+    *ints = plan_units(B) + z.max_units * UNIT;
     *slots = z.max_slots;
     return 0;
+}
+
+static int launch_plan(hipStream_t stream, const void* seq_lens, const void* leaders, const void* shared, void* plan,
+                       const PlanSizes& z) {
+    if (z.B <= 256)
+        hipLaunchKernelGGL(shared_plan_kernel<256>, dim3(1), dim3(256), 0, stream, (const int*)seq_lens,
+                           (const int*)leaders, (const int*)shared, (int*)plan, z);
+    else
+        hipLaunchKernelGGL(shared_plan_kernel<1024>, dim3(1), dim3(1024), 0, stream, (const int*)seq_lens,
+                           (const int*)leaders, (const int*)shared, (int*)plan, z);
+    HIP_CHECK_LAUNCH();
+    return 0;
+}
+
+static int shift_of(int block_size) {
+    return block_size >= 1 && (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
 }
 
 extern "C" int oa_shared_plan(void* stream, const void* seq_lens, const void* leaders, const void* shared, void* plan,
                               int B, int Hq, int Hk, int D, int width, int block_size) {
     if (!shared_sizes(B, Hq, Hk, D) || width < 1) return -100;
-    if (block_size < 1 || (block_size & (block_size - 1)) != 0) return -101;
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const int*)seq_lens,
-                       (const int*)leaders, (const int*)shared, (int*)plan,
-                       plan_sizes(B, Hq, Hk, width, __builtin_ctz(block_size)));
-    HIP_CHECK_LAUNCH();
-    return 0;
+    const int shift = shift_of(block_size);
+    if (shift < 0) return -101;
+    if ((uintptr_t)plan % 16 != 0) return -103;
+    return launch_plan((hipStream_t)stream, seq_lens, leaders, shared, plan, plan_sizes(B, Hq, Hk, width, shift));
 }
 
-// strides: q row, q head; k page, token, head; v page, token, head; table row: in elements
+// sizes: strides in elements (q row, q head; k page, token, head; v page, token, head; table row), then rows, heads,
+// key heads, channels, table width, pages, block size and whether the type is float16. leaders, shared, seq_lens:
+// null where `plan` is made already. scratch: floats, (D + 2) for each slot and head.
 extern "C" int oa_attention_decode_shared(void* stream, const void* q, const void* kc, const void* vc,
-                                          const void* block_table, const void* plan, void* o_part, void* ml_part,
-                                          void* out, const int64_t* strides, int B, int Hq, int Hk, int D, int pages,
-                                          int block_size, float scale, int f16) {
-    if (!shared_sizes(B, Hq, Hk, D) || pages < 1) return -100;
-    if (block_size < 1 || (block_size & (block_size - 1)) != 0) return -101;
-    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)o_part) % 16 != 0 || (uintptr_t)ml_part % 8 != 0) return -103;
+                                          const void* block_table, const void* seq_lens, const void* leaders,
+                                          const void* shared, void* plan, void* scratch, void* out,
+                                          const int64_t* sizes, float scale) {
+    const int64_t* const n = sizes + 9;
+    for (int i = 0; i < 7; ++i)
+        if (n[i] < 0 || n[i] > INT32_MAX) return -100;
+    const int B = (int)n[0], Hq = (int)n[1], Hk = (int)n[2], D = (int)n[3], width = (int)n[4], pages = (int)n[5];
+    const int shift = shift_of((int)n[6]);
+    if (!shared_sizes(B, Hq, Hk, D) || width < 1 || pages < 1) return -100;
+    if (shift < 0) return -101;
+    if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)plan | (uintptr_t)scratch) % 16 != 0) return -103;
     for (int i = 0; i < 8; ++i)
-        if (strides[i] % 8 != 0) return -103;
-    const PlanSizes z = plan_sizes(B, Hq, Hk, 1, 0);
+        if (sizes[i] % 8 != 0) return -103;
+    // a token's step is 24 bits in a transfer's offset
+    if (sizes[3] < 0 || sizes[3] >= (1 << 23) || sizes[6] < 0 || sizes[6] >= (1 << 23)) return -105;
+    const PlanSizes z = plan_sizes(B, Hq, Hk, width, shift);
+    const hipStream_t s = (hipStream_t)stream;
+    if (leaders) {
+        const int rc = launch_plan(s, seq_lens, leaders, shared, plan, z);
+        if (rc) return rc;
+    }
     SharedArgs a;
     a.q = (const char*)q;
     a.kc = (const char*)kc;
     a.vc = (const char*)vc;
     a.block_table = (const int*)block_table;
     a.plan = (const int*)plan;
-    a.o_part = (float*)o_part;
-    a.ml_part = (float*)ml_part;
+    a.o_part = (float*)scratch;
+    a.ml_part = a.o_part + (size_t)z.max_slots * Hq * D;
     int64_t* const steps[8] = {&a.q_row, &a.q_head, &a.k_page, &a.k_token, &a.k_head, &a.v_page, &a.v_token, &a.v_head};
-    for (int i = 0; i < 8; ++i) *steps[i] = strides[i] * 2;
-    a.table_row = strides[8];
+    for (int i = 0; i < 8; ++i) *steps[i] = sizes[i] * 2;
+    a.table_row = sizes[8];
     a.B = B;
     a.Hq = Hq;
     a.Hk = Hk;
     a.G = Hq / Hk;
     a.pages = pages;
-    a.shift = __builtin_ctz(block_size);
+    a.shift = shift;
     a.slots = z.max_slots;
     a.scale = scale * 1.44269504088896340736f;
-    const dim3 grid(z.max_units * Hk), merge(CEIL_DIV(B * Hq, 4)), block(256);
-#define LAUNCH(F16, DV, MT)                                                                                     \
-    hipLaunchKernelGGL((shared_attn_kernel<F16, DV, MT>), grid, block, 0, (hipStream_t)stream, a)
-#define LAUNCH_D(F16, DV)                                                                                       \
-    do {                                                                                                        \
-        if (z.tile == 16) LAUNCH(F16, DV, 1);                                                                   \
-        else if (z.tile == 32) LAUNCH(F16, DV, 2);                                                              \
-        else LAUNCH(F16, DV, 4);                                                                                \
-        HIP_CHECK_LAUNCH();                                                                                     \
-        hipLaunchKernelGGL((shared_combine_kernel<F16, DV>), merge, block, 0, (hipStream_t)stream, a.o_part,    \
-                           a.ml_part, a.plan, (char*)out, B, Hq, a.slots);                                      \
-        HIP_CHECK_LAUNCH();                                                                                     \
+    // four waves a (row, head) while that leaves every CU with little to do
+    const bool wide = B * Hq <= 1024;
+    const dim3 grid(z.runs * Hk), merge(wide ? B * Hq : CEIL_DIV(B * Hq, 4)), block(256);
+#define LAUNCH(F16, DV)                                                                                            \
+    do {                                                                                                           \
+        hipLaunchKernelGGL((shared_attn_kernel<F16, DV>), grid, block, 0, s, a);                                   \
+        HIP_CHECK_LAUNCH();                                                                                        \
+        if (wide)                                                                                                  \
+            hipLaunchKernelGGL((shared_combine_kernel<F16, DV, 4>), merge, block, 0, s, a.o_part, a.ml_part, a.plan, \
+                               (char*)out, B, Hq, a.slots);                                                        \
+        else                                                                                                       \
+            hipLaunchKernelGGL((shared_combine_kernel<F16, DV, 1>), merge, block, 0, s, a.o_part, a.ml_part, a.plan, \
+                               (char*)out, B, Hq, a.slots);                                                        \
+        HIP_CHECK_LAUNCH();                                                                                        \
     } while (0)
-    if (f16) {
-        if (D == 64) LAUNCH_D(true, 64);
-        else LAUNCH_D(true, 128);
+    if (n[7]) {
+        if (D == 64) LAUNCH(true, 64);
+        else LAUNCH(true, 128);
     } else {
-        if (D == 64) LAUNCH_D(false, 64);
-        else LAUNCH_D(false, 128);
+        if (D == 64) LAUNCH(false, 64);
+        else LAUNCH(false, 128);
     }
-#undef LAUNCH_D
 #undef LAUNCH
     return 0;
 }

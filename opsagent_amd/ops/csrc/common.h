@@ -94,6 +94,17 @@ __device__ __forceinline__ float wave_reduce_max(float v) {
     return v;
 }
 
+// inclusive sums over the wave's lanes, by row shifts and row broadcasts
+__device__ __forceinline__ int wave_sums(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // reduce within 16-lane groups (lanes differing only in bits 0..3)
 __device__ __forceinline__ float group16_reduce_sum(float v) {
 #pragma unroll

@@ -118,7 +118,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.oa_shared_plan_size.restype = i
     lib.oa_shared_plan.argtypes = [p, p, p, p, p, i, i, i, i, i, i]
     lib.oa_shared_plan.restype = i
-    lib.oa_attention_decode_shared.argtypes = [p] * 10 + [i] * 6 + [f, i]
+    lib.oa_attention_decode_shared.argtypes = [p] * 12 + [f]
     lib.oa_attention_decode_shared.restype = i
     lib.oa_kv_pages_copy.argtypes = [p, p, i, i64, i, i, i, p, i]
     lib.oa_kv_pages_copy.restype = i

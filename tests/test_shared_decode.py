@@ -355,7 +355,7 @@ def test_random_batches():
     (lambda c: c.update(block_table=c["block_table"][1:]), "rows"),
     (lambda c: c.update(seq_lens=c["seq_lens"].long()), "seq_lens"),
     (lambda c: c.update(leaders=c["leaders"][1:]), "leaders"),
-    (lambda c: c.update(shared=c["shared"].cpu()), "shared"),
+    (lambda c: c.update(shared=c["shared"].cpu()), "one device"),
     (lambda c: c.update(k_cache=c["k_cache"][:, :24], v_cache=c["v_cache"][:, :24]), "power of 2"),
     (lambda c: c.update(q=torch.empty(4 * 8 * 128 + 4, dtype=torch.bfloat16, device=DEVICE)[4:].view(4, 8, 128)),
      "16 bytes"),
