@@ -1685,7 +1685,7 @@ def kv_cache_copy(
         raise ValueError(f"{n} sources, {len(dst)} targets and {len(tokens)} numbers of tokens")
     if n == 0:
         return
-    if not all(isinstance(x, int) for part in (src, dst, tokens) for x in part):
+    if set(map(type, src + dst + tokens)) != {int}:
         raise TypeError("pages and tokens are ints on the host")
     if min(src) < 0 or max(src) >= last or min(dst) < 0 or max(dst) >= last:
         raise ValueError(f"page outside the cache of {last}")
@@ -1701,14 +1701,16 @@ def kv_cache_copy(
             for i in range(n):
                 t[dst[i], : tokens[i]] = t[src[i], : tokens[i]]
         return
+    if pages.device.index != torch.cuda.current_device():
+        with torch.cuda.device(pages.device):
+            return kv_cache_copy(pages, src, dst, tokens)
     lib, hip = _lib()
     flat = (ctypes.c_int * (3 * n))()
     flat[0::3], flat[1::3], flat[2::3] = src, dst, tokens
-    with torch.cuda.device(pages.device):
-        stream = hip.current_stream_ptr()
-        for bases, count, step, row in pages._launches:
-            hip.check(lib.oa_kv_pages_copy(stream, bases, count, step, row, block, last, flat, n),
-                      "oa_kv_pages_copy")
+    stream = hip.current_stream_ptr()
+    for bases, count, step, row in pages._launches:
+        hip.check(lib.oa_kv_pages_copy(stream, bases, count, step, row, block, last, flat, n),
+                  "oa_kv_pages_copy")
 
 
 def _prefill_splits(B: int, Hq: int, Hk: int, Sq: int, Skv: int) -> Tuple[int, bool]:

@@ -6,38 +6,33 @@
 // alone: read once, written once.
 //
 // Tables of bases and copies go with the launch, by value: nothing has to outlive the call, and a
-// captured launch keeps its own. Up to 192 tensors (the 160 of an 80-layer model) and 192 copies
-// fit in the 4 KiB that a launch may carry; more take more launches.
+// captured launch keeps its own. Up to 192 tensors (the 160 of an 80-layer model) and 128 copies
+// fit in the 4 KiB that a launch may carry; more take more launches. Copies of one source that
+// follow each other (a prompt's choices) read it once.
 
 #include "common.h"
 
-constexpr int MAX_TENSORS = 192, MAX_COPIES = 192;
+constexpr int MAX_TENSORS = 192, MAX_COPIES = 128;
 
 struct PageTensors {
     char* base[MAX_TENSORS];
 };
-struct PageCopies {
-    int src[MAX_COPIES], dst[MAX_COPIES], tokens[MAX_COPIES];
+struct PageCopies {                        // source i goes to dst[begin[i]] .. dst[begin[i + 1]]
+    int src[MAX_COPIES], tokens[MAX_COPIES], dst[MAX_COPIES];
+    uint16_t begin[MAX_COPIES + 1];
 };
 static_assert(sizeof(PageTensors) + sizeof(PageCopies) + 32 <= 4096, "what a launch may carry");
 
-// Grid: slices of a page, tensors, copies. A thread has UNROLL pieces of 16 bytes in flight.
-constexpr int UNROLL = 4;
+// Grid: 4-KiB slices of a page, tensors, sources.
 __global__ __launch_bounds__(256) void kv_pages_copy_kernel(PageTensors tensors, PageCopies copies,
                                                             int64_t step, int row) {
     char* const base = tensors.base[blockIdx.y];
     const int c = blockIdx.z;
-    const int64_t bytes = (int64_t)copies.tokens[c] * row;
-    const char* src = base + copies.src[c] * step;
-    char* dst = base + copies.dst[c] * step;
-    const int64_t at = ((int64_t)blockIdx.x * UNROLL * 256 + threadIdx.x) * 16;
-    uint4 part[UNROLL];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-        if (at + i * 4096 < bytes) part[i] = *reinterpret_cast<const uint4*>(src + at + i * 4096);
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-        if (at + i * 4096 < bytes) *reinterpret_cast<uint4*>(dst + at + i * 4096) = part[i];
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+    if (at >= (int64_t)copies.tokens[c] * row) return;
+    const uint4 piece = *reinterpret_cast<const uint4*>(base + copies.src[c] * step + at);
+    for (int i = copies.begin[c]; i < copies.begin[c + 1]; ++i)
+        *reinterpret_cast<uint4*>(base + copies.dst[i] * step + at) = piece;
 }
 
 // bases: `tensors` addresses on the host, each of `pages` pages `step` bytes apart, a page `block`
@@ -60,18 +55,21 @@ extern "C" int oa_kv_pages_copy(void* stream, const uint64_t* bases, int tensors
         for (int c0 = 0; c0 < n; c0 += MAX_COPIES) {
             const int nc = min(MAX_COPIES, n - c0);
             PageCopies c;
-            int most = 0;
+            int sources = 0, most = 0;
             for (int i = 0; i < nc; ++i) {
                 const int* p = copies + 3 * (c0 + i);
-                c.src[i] = p[0];
+                if (!sources || c.src[sources - 1] != p[0] || c.tokens[sources - 1] != p[2]) {
+                    c.src[sources] = p[0];
+                    c.tokens[sources] = p[2];
+                    c.begin[sources++] = (uint16_t)i;
+                }
                 c.dst[i] = p[1];
-                c.tokens[i] = p[2];
                 most = max(most, p[2]);
             }
+            c.begin[sources] = (uint16_t)nc;
             if (!most) continue;
-            const int64_t slices = CEIL_DIV((int64_t)most * row, UNROLL * 4096);
-            hipLaunchKernelGGL(kv_pages_copy_kernel, dim3((unsigned)slices, nt, nc), dim3(256), 0,
-                               (hipStream_t)stream, t, c, step, row);
+            hipLaunchKernelGGL(kv_pages_copy_kernel, dim3((unsigned)CEIL_DIV((int64_t)most * row, 4096), nt, sources),
+                               dim3(256), 0, (hipStream_t)stream, t, c, step, row);
             HIP_CHECK_LAUNCH();
         }
     }
