@@ -1707,7 +1707,7 @@ def kv_cache_copy(
     lib, hip = _lib()
     flat = (ctypes.c_int * (3 * n))()
     flat[0::3], flat[1::3], flat[2::3] = src, dst, tokens
-    stream = hip.current_stream_ptr()
+    stream = hip.stream_ptr(pages.device.index)
     for bases, count, step, row in pages._launches:
         hip.check(lib.oa_kv_pages_copy(stream, bases, count, step, row, block, last, flat, n),
                   "oa_kv_pages_copy")
@@ -2016,7 +2016,8 @@ def attention_decode_shared(
     that shares nothing leads itself; so does one whose leader is no row that leads itself, or has
     no keys. A group shares as many pages as all of its rows do, full ones only; what some of its
     rows share beyond that is read for each. ``plan``: of shared_decode_plan for these lengths and
-    leaders, made here where it is None. No gradients."""
+    leaders; where it is None, a launch of up to 64 rows makes its own, and one of more is preceded by
+    one that does. No gradients."""
     if not _is_gpu(q):
         return torch_ref.attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders,
                                                  shared, scale)
@@ -2041,11 +2042,11 @@ def attention_decode_shared(
             return attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders, shared,
                                            scale, plan)
     lib, hip = _lib()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    room = torch.empty(floats + (ints if plan is None else 0), dtype=torch.float32, device=q.device)
+    out = q.new_empty(q.shape)
+    room = q.new_empty(floats + (ints if plan is None else 0), dtype=torch.float32)
     start = room.data_ptr()
     rc = lib.oa_attention_decode_shared(
-        hip.current_stream_ptr(), *at, block_table.data_ptr(),
+        hip.stream_ptr(device), *at, block_table.data_ptr(),
         *((seq_lens.data_ptr(), leaders.data_ptr(), shared.data_ptr(), start) if plan is None
           else (None, None, None, plan.ints.data_ptr())),
         start + 4 * ints if plan is None else start, out.data_ptr(), sizes,

@@ -58,6 +58,7 @@ __device__ __forceinline__ uint32_t sh_pack(float lo, float hi) {
 constexpr int PLAN_HEAD = 8, UNIT = 8, UNIT_COST = 1;
 constexpr int PLAN_ROWS = 2048;
 constexpr int TILE = 128;                          // columns that a block takes
+constexpr int SIZES = 8;                           // sizes of an item that are looked at
 
 struct PlanSizes {
     int B, G, width, shift, tile, runs, max_units, max_slots;    // tile: members of TILE columns
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restr
                                                               const int* __restrict__ leaders,
                                                               const int* __restrict__ shared,
                                                               int* __restrict__ plan, PlanSizes z) {
-    constexpr int ROWS = THREADS == 1024 ? PLAN_ROWS : THREADS, NW = THREADS / WAVE, SIZES = 8;
+    constexpr int ROWS = THREADS == 1024 ? PLAN_ROWS : THREADS, NW = THREADS / WAVE;
     // of a row: keys, leader, keys behind the shared ones, place in the line, chunks of the shared
     // ones, first slot; of a leader: members, common keys, places in members and among the units
     __shared__ int keys[ROWS], lead[ROWS], rests[ROWS], chunks[ROWS], slot_of[ROWS], count[ROWS], common[ROWS],
@@ -270,19 +271,113 @@ __global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restr
 // ---- attention ---------------------------------------------------------------------------------
 struct SharedArgs {
     const char *q, *kc, *vc;
-    const int* block_table;
-    const int* plan;
+    const int *block_table, *seq_lens, *leaders, *shared;
+    int* plan;
     float *o_part, *ml_part;
     int64_t q_row, q_head, k_page, k_token, k_head, v_page, v_token, v_head;     // bytes
     int64_t table_row;
     int B, Hq, Hk, G, pages, shift, slots;
     float scale;                                                                 // times log2(e)
+    PlanSizes z;
 };
+
+constexpr int IDS = 1024;                          // pages of a unit that lie in LDS at a time
+
+// what a block keeps in LDS of its item: the pages of a unit's keys; rows and slots of a group's tile;
+// of a plan made here, the first unit and each row's first unit
+struct SharedPlaces {
+    int ids[IDS], rows[TILE], slots[TILE];
+};
+struct OwnPlan {
+    int4 first[2];                                 // row (-1: none), first key, end, members | slot, next row, items
+    int4 row[WAVE];                                // first key, end, slot, next row
+    int count[WAVE], common[WAVE];
+};
+
+// The plan of up to 64 rows, as shared_plan_kernel makes it, by one wave for itself: a lane a row. It
+// takes a microsecond of every block, and a launch before this one 10 (with its wait for the chip).
+__device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan& own, SharedPlaces& places) {
+    const PlanSizes& z = a.z;
+    const int lane = threadIdx.x & (WAVE - 1), B = z.B;
+    const bool in = lane < B;
+    const int most = (int)min((int64_t)z.width << z.shift, (int64_t)INT32_MAX - 4096);
+    const int keys = in ? min(max(a.seq_lens[lane], 0), most) : 0;
+    const int l = in ? a.leaders[lane] : lane, sh = in ? a.shared[lane] : 0;
+    own.count[lane] = 0;
+    own.common[lane] = INT32_MAX;
+    const int l_of = __shfl(l, l & (WAVE - 1), WAVE), l_keys = __shfl(keys, l & (WAVE - 1), WAVE);
+    const bool led = in && (uint32_t)l < (uint32_t)B && l != lane && l_of == l && keys > 0 && l_keys > 0;
+    const int to = led ? l : lane, pages = keys >> z.shift;
+    atomicAdd(&own.count[to], 1);
+    atomicMin(&own.common[to], led ? min(max(sh, 0), pages) : pages);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int count = own.count[lane], common = count > 1 ? own.common[lane] << z.shift : 0;
+    const int tiles = (int)cdiv(count, z.tile);
+    const int p = __shfl(common, to, WAVE), rest = keys - p;
+    auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_sums(v), WAVE - 1); };
+    const uint32_t cost = rest > 0 ? in_sizes(rest) + UNIT_COST : 0, sums = wave_sums(cost), line = sums - cost;
+    const uint32_t behind = __builtin_amdgcn_readlane(sums, WAVE - 1);
+    const uint32_t all = behind + wave_total(common ? tiles * (in_sizes(common) + UNIT_COST) : 0);
+    const uint32_t share = max(2u, cdiv(all, (uint32_t)z.runs));
+    uint32_t run = share;
+    for (int i = 0; i < SIZES; ++i) {
+        run = share + share * i / (2 * SIZES);
+        const int n = wave_total(common ? tiles * about_chunks(common, 1.0f / run) : 0);
+        if (n + cdiv(behind, run) <= (uint32_t)z.runs) break;
+    }
+    const float per_run = 1.0f / run;
+    const int chunk = common ? plan_chunk(common, per_run) : 1, chunks = common ? (int)cdiv(common, chunk) : 0;
+    const int nu = tiles * chunks, iu = wave_sums(nu), unit_of = iu - nu, ahead = __builtin_amdgcn_readlane(iu, WAVE - 1);
+    int lines = (int)cdiv(behind, run);
+    if (behind > 0 && ahead + lines < z.runs) lines = (int)min((uint32_t)(z.runs - ahead), max(behind / 2, 1u));
+    const uint32_t step = lines > 0 ? max(2u, cdiv(behind, lines)) : 1;
+    if (lines > 0) lines = (int)cdiv(behind, step);
+    const int from = (int)cdiv(line + 1, step);
+    const int upto = rest > 0 ? (int)cdiv(line + 2 * ((uint32_t)(rest + 127) >> 7) - 1, step) : 0;
+    auto cut = [&](int i) { return (int)((i * step - line + 1) >> 1 << 7); };
+    const int shared_chunks = __shfl(chunks, to, WAVE);
+    const int splits = shared_chunks + (rest > 0 ? 1 + upto - from : 0), slot = wave_sums(splits) - splits;
+    if (blockIdx.x == 0 && in) {                             // for the combine
+        a.plan[PLAN_HEAD + lane] = slot;
+        a.plan[PLAN_HEAD + B + lane] = splits;
+    }
+    const uint64_t live = __ballot(rest > 0), below = live & ((1ull << lane) - 1), above = live & ~((2ull << lane) - 1);
+    const int ended = __shfl(upto, below ? 63 - __builtin_clzll(below) : 0, WAVE), before = below ? ended : 0;
+    const int next = above ? __builtin_ctzll(above) : 0, next_from = __shfl(from, next, WAVE);
+    const int link = above && next_from == upto ? next : -1;
+    const int start = p + (from < upto ? cut(from) : rest), start_link = from < upto ? -1 : link;
+    own.row[lane] = int4{p, start, slot + shared_chunks, start_link};
+    if (lane == 0) own.first[0] = int4{-1, 0, 0, 0};
+    if (lane == 0) own.first[1] = int4{0, -1, ahead + lines, 0};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (item < ahead) {
+        const int lead = __builtin_ctzll(__ballot(unit_of <= item && item < unit_of + nu));
+        auto of_lead = [&](int v) { return __builtin_amdgcn_readlane(v, lead); };
+        const int i = item - of_lead(unit_of), n = of_lead(tiles), part = i / n, at = i % n * z.tile, c = of_lead(chunk);
+        const int members = min(z.tile, of_lead(count) - at);
+        const bool mine = in && to == lead;
+        const uint64_t all_mine = __ballot(mine);
+        const int rank = __builtin_popcountll(all_mine & ((1ull << lane) - 1)) - at;
+        if (mine && rank >= 0 && rank < members) {
+            places.rows[rank] = lane;
+            places.slots[rank] = slot + part;
+        }
+        if (lane == lead) own.first[0] = int4{lead, part * c, min(part * c + c, common), members};
+    } else {
+        const int i = item - ahead;
+        if (rest > 0 && i == from - 1 && before < from) {
+            own.first[0] = int4{lane, p, start, 0};
+            own.first[1] = int4{slot + shared_chunks, start_link, ahead + lines, 0};
+        } else if (rest > 0 && i >= from && i < upto) {
+            own.first[0] = int4{lane, p + cut(i), p + (i + 1 < upto ? cut(i + 1) : rest), 0};
+            own.first[1] = int4{slot + shared_chunks + 1 + i - from, i + 1 < upto ? -1 : link, ahead + lines, 0};
+        }
+    }
+}
 
 struct SharedUnit {
-    int row, begin, end, place, group, split, slot, columns;
+    int row, begin, end, group, slot, columns;     // group: members, their rows and slots in LDS
 };
-
 // Four waves take a unit's chunk for one key head. A wave has up to 32 columns (MT tiles of 16), so
 // KG groups of waves share the keys out, 32 in turn, and the 4 / KG waves of a group the columns:
 //     columns     up to 32     64     128
@@ -300,8 +395,6 @@ struct SharedUnit {
 // 16-byte pieces of key rows and 32-byte pieces of value rows change places with the key, so that
 // neither the reads of key rows nor the transposing ones meet in a bank; a transfer writes LDS in
 // lane order, so its source address carries the change.
-constexpr int IDS = 1024;                          // pages of a unit that lie in LDS at a time
-
 template <int N>
 __device__ __forceinline__ void wait_transfers() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
@@ -323,7 +416,7 @@ __device__ __forceinline__ float over_groups(float v) {
 }
 
 template <bool F16, int D, int MT, int KG>
-__device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUnit& unit, int h, char* lds) {
+__device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUnit& unit, int h, char* lds, SharedPlaces& places) {
     constexpr int NS = D / 32, ND = D / 16, ROW = D * 2, CPR = ROW / 16;
     constexpr int CG = 4 / KG, KEYS = KG == 1 ? 64 : 32, STAGES = KG == 4 ? 1 : 2;
     constexpr int PLANE = KEYS * ROW, STAGE = 2 * PLANE, NJ = KEYS / 16;
@@ -335,14 +428,9 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int kg = wave / CG, cg = wave % CG;
     const int row0 = unit.row, begin = unit.begin, end = unit.end, columns = unit.columns;
-    const int* const members = unit.group ? a.plan + PLAN_HEAD + 2 * a.B + unit.place : nullptr;
     const int G = a.G, mask = (1 << a.shift) - 1;
-    constexpr int RING = 4 * 32 * D * 4, MERGE = 4 * 32 * (D + 4 + 2) * 4;
-    int* const ids = reinterpret_cast<int*>(lds + (RING > MERGE ? RING : MERGE));
-    int* const slots = ids + IDS;                            // of the tile's members
-    const int* const first = a.plan + PLAN_HEAD;
-    if (members)
-        for (int i = threadIdx.x; i < unit.group; i += 256) slots[i] = first[members[i]];
+    constexpr int RING = 4 * 32 * D * 4;
+    int* const ids = places.ids;
     char* const ring = lds + kg * (RING / KG);
     const uint32_t ring_at = (uint32_t)(uintptr_t)ring;
 
@@ -351,20 +439,23 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     // signs of q so that larger products are larger weights; no q at all where the scale is 0
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep_q = a.scale == 0.0f ? 0u : ~0u;
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+    auto load_q = [&](bool group) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int c = cg * 32 + m * 16 + col;
-        const bool in = c < columns;
-        const int cc = in ? c : 0;
-        const int b = members ? members[cc / G] : row0;
-        const char* at = a.q + b * a.q_row + (h * G + cc % G) * a.q_head + g * 16;
+        for (int m = 0; m < MT; ++m) {
+            const int c = cg * 32 + m * 16 + col;
+            const bool in = c < columns;
+            const int cc = in ? c : 0;
+            const char* at = group ? a.q + places.rows[cc / G] * a.q_row + (h * G + cc % G) * a.q_head + g * 16
+                                   : a.q + row0 * a.q_row + (h * G + cc) * a.q_head + g * 16;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const uint4 w = *reinterpret_cast<const uint4*>(at + s * 64);
-            qf[m][s] = in ? uint4{(w.x ^ flip) & keep_q, (w.y ^ flip) & keep_q, (w.z ^ flip) & keep_q, (w.w ^ flip) & keep_q}
-                          : uint4{0, 0, 0, 0};
+            for (int s = 0; s < NS; ++s) {
+                const uint4 w = *reinterpret_cast<const uint4*>(at + s * 64);
+                qf[m][s] = in ? uint4{(w.x ^ flip) & keep_q, (w.y ^ flip) & keep_q, (w.z ^ flip) & keep_q, (w.w ^ flip) & keep_q}
+                              : uint4{0, 0, 0, 0};
+            }
         }
-    }
+    };
+    if (!unit.group) load_q(false);                          // a group's rows are known behind the barrier
     sh_f4 o[MT][ND];
     // sums of weights come from the matrix cores too, as the product with values of 1: of the rounded
     // weights, which the outputs are made of
@@ -428,9 +519,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
         }
     };
 
-    // a step's keys from LDS: scores, weights, and their product with the values. The first values are
-    // read ahead of the weights.
-    constexpr int EARLY = ND / 2;
+    // a step's keys from LDS: scores, weights, and their product with the values
     uint4 pf[MT][NJ / 2];
     sh_f4 sc[MT][NJ];
     auto products = [&](const char* kt) {
@@ -499,22 +588,23 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
         v.p.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)hi);
         return v.u;
     };
-    auto add_values = [&](const char* vt, const uint4* early) {
+    auto add_values = [&](const char* vt) {
 #pragma unroll
         for (int half = 0; half < NJ / 2; ++half) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) sum[m] = sh_product<F16>(ones, pf[m][half], sum[m]);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const uint4 v = early && half == 0 && d < EARLY ? early[d] : value(vt, half, d);
+                const uint4 v = value(vt, half, d);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) o[m][d] = sh_product<F16>(v, pf[m][half], o[m][d]);
             }
         }
     };
 
+    __syncthreads();                                         // the places
+    if (unit.group) load_q(true);
     for (;;) {
-    __syncthreads();                                         // ids
     if constexpr (KG == 4) {
         int key = k0 + kg * 32;
         if (key < k1) {
@@ -530,7 +620,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             weights(key);
             if (more) wait_transfers<PCS>();
             else wait_transfers<0>();
-            add_values(ring + PLANE, nullptr);
+            add_values(ring + PLANE);
             wait_reads();
             if (more) load_rows(true, key + 128, ring_at + PLANE);
         }
@@ -557,11 +647,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             const char* const at = ring + i % STAGES * STAGE;
             if (busy && i < mine) {
                 products(at);
-                uint4 early[EARLY];
-#pragma unroll
-                for (int d = 0; d < EARLY; ++d) early[d] = value(at + PLANE, 0, d);
                 weights(key_of(i));
-                add_values(at + PLANE, early);
+                add_values(at + PLANE);
             }
         }
     }
@@ -570,6 +657,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     k0 = k1;
     k1 = k0 + min(span, end - k0);
     place_pages();
+    __syncthreads();
     }
 
     // a common maximum of the groups' sums of each column, in units of the weights' exponent
@@ -606,7 +694,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             l += st[w].y * f;
             acc += *reinterpret_cast<const sh_f4*>(merge + (w * COLS + c) * PITCH + ch) * f;
         }
-        const int slot = (members ? slots[c / G] : unit.slot) + unit.split;
+        const int slot = unit.group ? places.slots[c / G] : unit.slot;
         if (slot >= a.slots) continue;
         const size_t to = (size_t)slot * a.Hq + h * G + c % G;
         *reinterpret_cast<sh_f4*>(a.o_part + to * D + ch) = acc;
@@ -614,37 +702,70 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     }
 }
 
-// Grid: units times key heads, the heads of a unit side by side: with eight of them a key head is on
-// one die, whose L2 then has a chunk for all tiles of columns.
-template <bool F16, int D>
+// Grid: `runs` blocks for each key head, the heads of an item side by side: with eight of them a key
+// head is on one die, whose L2 then has a chunk for all tiles of columns. PLANNED: by a plan made
+// before; else of up to 64 rows, by one that the block makes.
+template <bool F16, int D, bool PLANNED>
 __global__ __launch_bounds__(256, 2) void shared_attn_kernel(SharedArgs a) {
     constexpr int RING = 4 * 32 * D * 4, MERGE = 4 * 32 * (D + 4 + 2) * 4;
-    __shared__ __attribute__((aligned(16))) char lds[(RING > MERGE ? RING : MERGE) + (IDS + TILE) * 4];
-    const int h = blockIdx.x % a.Hk;
-    const int* const units = a.plan + plan_units(a.B);
-    // the number of items and the first one's record in one wait: there is room for `runs` of them
-    const int4* const mine = reinterpret_cast<const int4*>(units) + 2 * (size_t)(blockIdx.x / a.Hk);
-    const int count = a.plan[0];
-    int4 x = mine[0], y = mine[1];
-    const int items = __builtin_amdgcn_readfirstlane(count);
-    for (int i = blockIdx.x / a.Hk; i < items; i += gridDim.x / a.Hk)
-        for (int u = i; u >= 0;) {
-            if (u != (int)(blockIdx.x / a.Hk)) {
-                const int4* const at = reinterpret_cast<const int4*>(units) + 2 * (size_t)u;
-                x = at[0];
-                y = at[1];
+    __shared__ __attribute__((aligned(16))) char lds[RING > MERGE ? RING : MERGE];
+    __shared__ SharedPlaces places;
+    const int h = blockIdx.x % a.Hk, begin = blockIdx.x / a.Hk;
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    auto take = [&](const SharedUnit& unit) {
+        if (unit.columns <= 16) shared_unit<F16, D, 1, 4>(a, unit, h, lds, places);
+        else if (unit.columns <= 32) shared_unit<F16, D, 2, 4>(a, unit, h, lds, places);
+        else if (unit.columns <= 64) shared_unit<F16, D, 2, 2>(a, unit, h, lds, places);
+        else shared_unit<F16, D, 2, 1>(a, unit, h, lds, places);
+        __syncthreads();                                     // LDS is the next unit's
+    };
+    if constexpr (PLANNED) {
+        const int* const first = a.plan + PLAN_HEAD;
+        const int* const members = first + 2 * a.B;
+        const int4* const units = reinterpret_cast<const int4*>(a.plan + plan_units(a.B));
+        // the number of items and the first one's record in one wait: there is room for `runs` of them
+        const int count = a.plan[0];
+        int4 x = units[2 * (size_t)begin], y = units[2 * (size_t)begin + 1];
+        const int items = same(count);
+        for (int i = begin; i < items; i += a.z.runs)
+            for (int u = i; u >= 0;) {
+                if (u != begin) {
+                    x = units[2 * (size_t)u];
+                    y = units[2 * (size_t)u + 1];
+                }
+                const int place = same(x.w), split = same(y.y);
+                SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(y.x), same(y.w) + split, 0};
+                unit.columns = max(unit.group, 1) * a.G;
+                u = same(y.z);
+                if ((uint32_t)unit.row >= (uint32_t)a.B) continue;   // an item without units
+                for (int j = threadIdx.x; j < unit.group; j += 256) {
+                    const int b = members[place + j];
+                    places.rows[j] = b;
+                    places.slots[j] = first[b] + split;
+                }
+                take(unit);
             }
-            auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-            SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(x.w), same(y.x), same(y.y), same(y.w), 0};
-            const int columns = unit.columns = max(unit.group, 1) * a.G;
-            u = same(y.z);
-            if ((uint32_t)unit.row >= (uint32_t)a.B) continue;   // an item without units
-            if (columns <= 16) shared_unit<F16, D, 1, 4>(a, unit, h, lds);
-            else if (columns <= 32) shared_unit<F16, D, 2, 4>(a, unit, h, lds);
-            else if (columns <= 64) shared_unit<F16, D, 2, 2>(a, unit, h, lds);
-            else shared_unit<F16, D, 2, 1>(a, unit, h, lds);
-            __syncthreads();                                 // LDS is the next unit's
+    } else {
+        __shared__ OwnPlan own;
+        for (int i = begin;; i += a.z.runs) {
+            if (threadIdx.x < WAVE) plan_item(a, i, own, places);
+            __syncthreads();
+            int4 x = own.first[0];
+            const int4 y = own.first[1];
+            const int items = same(y.z);
+            SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(x.w), same(y.x), 0};
+            unit.columns = max(unit.group, 1) * a.G;
+            for (int next = same(y.y); (uint32_t)unit.row < (uint32_t)a.B;) {
+                take(unit);
+                if (next < 0) break;
+                x = own.row[next];
+                unit = SharedUnit{next, same(x.x), same(x.y), 0, same(x.z), a.G};
+                next = same(x.w);
+            }
+            if (i + a.z.runs >= items) break;
+            __syncthreads();                                 // all have read the item
         }
+    }
 }
 
 // PER waves take a (row, head): the slots' sums with their common maximum. Weights of up to 64 slots
@@ -806,7 +927,8 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     if (sizes[3] < 0 || sizes[3] >= (1 << 23) || sizes[6] < 0 || sizes[6] >= (1 << 23)) return -105;
     const PlanSizes z = plan_sizes(B, Hq, Hk, width, shift);
     const hipStream_t s = (hipStream_t)stream;
-    if (leaders) {
+    const bool planned = !leaders || B > WAVE;
+    if (leaders && planned) {
         const int rc = launch_plan(s, seq_lens, leaders, shared, plan, z);
         if (rc) return rc;
     }
@@ -815,7 +937,11 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     a.kc = (const char*)kc;
     a.vc = (const char*)vc;
     a.block_table = (const int*)block_table;
-    a.plan = (const int*)plan;
+    a.seq_lens = (const int*)seq_lens;
+    a.leaders = (const int*)leaders;
+    a.shared = (const int*)shared;
+    a.plan = (int*)plan;
+    a.z = z;
     a.o_part = (float*)scratch;
     a.ml_part = a.o_part + (size_t)z.max_slots * Hq * D;
     int64_t* const steps[8] = {&a.q_row, &a.q_head, &a.k_page, &a.k_token, &a.k_head, &a.v_page, &a.v_token, &a.v_head};
@@ -834,7 +960,8 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     const dim3 grid(z.runs * Hk), merge(wide ? B * Hq : CEIL_DIV(B * Hq, 4)), block(256);
 #define LAUNCH(F16, DV)                                                                                            \
     do {                                                                                                           \
-        hipLaunchKernelGGL((shared_attn_kernel<F16, DV>), grid, block, 0, s, a);                                   \
+        if (planned) hipLaunchKernelGGL((shared_attn_kernel<F16, DV, true>), grid, block, 0, s, a);                \
+        else hipLaunchKernelGGL((shared_attn_kernel<F16, DV, false>), grid, block, 0, s, a);                       \
         HIP_CHECK_LAUNCH();                                                                                        \
         if (wide)                                                                                                  \
             hipLaunchKernelGGL((shared_combine_kernel<F16, DV, 4>), merge, block, 0, s, a.o_part, a.ml_part, a.plan, \

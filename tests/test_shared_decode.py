@@ -118,6 +118,9 @@ def test_groups(name, Hq, Hk, D, bs, dtype):
     rows = _at_block(GROUPS[name], bs)
     c = _case(rows, Hq, Hk, D, bs, dtype, seed=len(name))
     _check(ops.attention_decode_shared(**c), c)
+    plan = ops.shared_decode_plan(c["seq_lens"], c["leaders"], c["shared"], (Hq, Hk), D,
+                                  c["block_table"].shape[1], bs)
+    _check(ops.attention_decode_shared(**c, plan=plan), c)
 
 
 @gpu
