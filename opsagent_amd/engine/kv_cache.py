@@ -17,9 +17,13 @@ cached (refcount 0) in LRU order and are evicted on allocation pressure.
 from __future__ import annotations
 
 import collections
+import functools
+import itertools
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
+
+from opsagent_amd import ops
 
 
 class BlockAllocatorError(RuntimeError):
@@ -89,6 +93,80 @@ class PagedKVCache:
         # LRU of refcount-0 cached blocks (evictable)
         self._evictable: "collections.OrderedDict[int, None]" = collections.OrderedDict()
         self.stats = {"reused_blocks": 0, "allocated_blocks": 0, "evictions": 0}
+        self._pages: Optional[ops.KVPages] = None
+        self.switched = 0       # blocks that sequences gave up for an equal published one
+
+    # -- contents of blocks -------------------------------------------------
+    def copy_blocks(self, src: Sequence[int], dst: Sequence[int],
+                    tokens: Optional[Sequence[int]] = None) -> None:
+        """Keys and values of blocks src to blocks dst in all layers, or of their first tokens."""
+        if len(src):
+            if self._pages is None:
+                self._pages = ops.KVPages(self.layers)
+            ops.kv_cache_copy(self._pages, src, dst, tokens)
+
+    def drop_cached(self, keep: int = 0) -> int:
+        """Frees blocks that only the prefix cache holds, the longest unused first, until `keep` of
+        them are left. Returns how many were freed."""
+        drop = max(0, len(self._evictable) - max(0, keep))
+        for _ in range(drop):
+            bid, _ = self._evictable.popitem(last=False)
+            self._forget(bid)
+            self._free.append(bid)
+        return drop
+
+    def compact(self, sequences: Sequence["SequenceState"]) -> int:
+        """Moves what is in use or cached to the first blocks, so that the rest of the pool is one
+        run of free blocks; returns where that begins. `sequences` are all that hold blocks: their
+        lists are changed. Nothing may be reading or writing the cache on another stream."""
+        held = collections.Counter(b for seq in sequences for b in seq.blocks)
+        if any(seq.cache is not self for seq in sequences) or any(
+                self._ref[b] != held[b] for b in range(self.num_blocks)):
+            raise ValueError("compacting takes every sequence that holds blocks of the cache")
+        used = [b for b in range(self.num_blocks) if self._ref[b] or b in self._evictable]
+        n, taken = len(used), set(used)
+        src = [b for b in used if b >= n]
+        dst = [b for b in range(n) if b not in taken]
+        self.copy_blocks(src, dst)
+        to = dict(zip(src, dst))
+        for a, b in to.items():
+            self._ref[a], self._ref[b] = 0, self._ref[a]
+            self._block_tokens[a], self._block_tokens[b] = None, self._block_tokens[a]
+            h, self._block_to_hash[a] = self._block_to_hash[a], None
+            self._block_to_hash[b] = h
+            if h is not None:
+                self._hash_to_block[h] = b
+        self._evictable = collections.OrderedDict((to.get(b, b), None) for b in self._evictable)
+        self._free = collections.deque(range(n, self.num_blocks))
+        for seq in sequences:
+            seq.blocks = [to.get(b, b) for b in seq.blocks]
+        return n
+
+    def shrink(self, num_blocks: int, sequences: Sequence["SequenceState"]) -> None:
+        """Gives memory back: the pool becomes its first `num_blocks`, compacted, cached blocks that
+        find no room dropped. The layers' tensors are new ones. Raises BlockAllocatorError where
+        sequences hold more blocks than that."""
+        if not 0 < num_blocks <= self.num_blocks:
+            raise ValueError(f"a pool of {self.num_blocks} blocks does not shrink to {num_blocks}")
+        live = sum(1 for r in self._ref if r)
+        if live > num_blocks:
+            raise BlockAllocatorError(f"{live} blocks are in use, more than {num_blocks}")
+        self.drop_cached(num_blocks - live)
+        self.compact(sequences)
+        self._pages = None
+        for i, (k, v) in enumerate(self.layers):
+            if k is None:
+                continue
+            # layer by layer: the peak is one layer more than the pool
+            self.layers[i] = (None, None)
+            prefix = v.data_ptr() == k.data_ptr()
+            vdim, keys = v.shape[-1], k[:num_blocks].clone()
+            values = keys[..., :vdim] if prefix else v[:num_blocks].clone()
+            del k, v
+            self.layers[i] = (keys, values)
+        del self._ref[num_blocks:], self._block_to_hash[num_blocks:], self._block_tokens[num_blocks:]
+        self._free = collections.deque(b for b in self._free if b < num_blocks)
+        self.num_blocks = num_blocks
 
     # -- low-level allocator ----------------------------------------------
     def num_free(self) -> int:
@@ -99,14 +177,18 @@ class PagedKVCache:
             return self._free.popleft()
         if self._evictable:
             bid, _ = self._evictable.popitem(last=False)  # LRU
-            h = self._block_to_hash[bid]
-            if h is not None:
-                del self._hash_to_block[h]
-                self._block_to_hash[bid] = None
-                self._block_tokens[bid] = None
+            self._forget(bid)
             self.stats["evictions"] += 1
             return bid
         raise BlockAllocatorError("KV cache out of blocks")
+
+    def _forget(self, bid: int) -> None:
+        """Takes a block out of the prefix cache's tables."""
+        h = self._block_to_hash[bid]
+        if h is not None:
+            del self._hash_to_block[h]
+            self._block_to_hash[bid] = None
+            self._block_tokens[bid] = None
 
     def alloc_block(self) -> int:
         bid = self._pop_free_block()
@@ -170,6 +252,7 @@ class PagedKVCache:
             if self._block_tokens[existing] == prefix_tokens:
                 self.retain(existing)
                 self.release(bid)
+                self.switched += 1
                 return existing
             # hash collision with DIFFERENT content: evict the stale entry
             self._block_to_hash[existing] = None
@@ -218,6 +301,69 @@ class StateSlotPool:
         self._free.append(slot)
 
 
+def shared_prefixes(
+    tables: Sequence[Sequence[int]], full: Sequence[int]
+) -> Tuple[List[int], List[int], int]:
+    """Which rows of a batch begin with the same blocks, as ops.attention_decode_shared takes it:
+    (leaders, shared, saved). `tables`: block ids of each row; `full`: how many of them are full.
+    Rows are grouped so that the blocks read once instead of once a row are as many as one level of
+    groups allows; `saved` is their number."""
+    n = len(tables)
+    leaders, shared, saved = list(range(n)), [0] * n, 0
+    order = sorted(range(n), key=lambda b: list(tables[b][: full[b]]))
+    # blocks in common of neighbours in that order; of a run of rows, the least of them
+    common = []
+    for a, b in zip(order, order[1:]):
+        most, same = min(full[a], full[b]), 0
+        ta, tb = tables[a], tables[b]
+        while same < most and ta[same] == tb[same]:
+            same += 1
+        common.append(same)
+
+    # A group reads its blocks once, and each of its rows less by as many. Runs of rows with blocks in
+    # common are a tree; a run is a group or not, and rows go to the nearest group around them.
+    @functools.lru_cache(maxsize=None)
+    def best(lo: int, hi: int, around: int) -> Tuple[int, bool]:
+        """Blocks that rows lo..hi read less in a group of `around` blocks, or in better ones within
+        it; whether the run is a group of its own."""
+        if hi - lo == 1:
+            return around, False
+        least, parts = cut(lo, hi)
+        rest = sum(best(*p, around)[0] for p in parts)
+        own = sum(best(*p, least)[0] for p in parts) - least if least > around else rest
+        return (own, True) if own > rest else (rest, False)
+
+    @functools.lru_cache(maxsize=None)
+    def cut(lo: int, hi: int) -> Tuple[int, List[Tuple[int, int]]]:
+        least = min(common[lo : hi - 1])
+        edges = [lo] + [i + 1 for i in range(lo, hi - 1) if common[i] == least] + [hi]
+        return least, list(zip(edges, edges[1:]))
+
+    # (run, blocks of the group around it, its rows); runs of 256 rows bound the depth
+    groups: List[Tuple[int, List[int]]] = []
+    work = [(lo, min(lo + 256, n), 0, None) for lo in range(0, n, 256)]
+    while work:
+        lo, hi, around, rows = work.pop()
+        if hi - lo == 1:
+            if rows is not None:
+                rows.append(order[lo])
+            continue
+        least, parts = cut(lo, hi)
+        if best(lo, hi, around)[1]:
+            around, rows = least, []
+            groups.append((least, rows))
+        work.extend((*part, around, rows) for part in parts)
+    for pages, rows in groups:
+        if len(rows) > 1:
+            saved += (len(rows) - 1) * pages
+            for b in rows:
+                leaders[b], shared[b] = min(rows), pages
+    return leaders, shared, saved
+
+
+_SERIAL = itertools.count()
+
+
 class SequenceState:
     """Per-sequence cache bookkeeping."""
 
@@ -234,6 +380,33 @@ class SequenceState:
         self.num_cached = 0     # tokens whose KV is in cache
         self.chain_h = 0        # chain hash over published full blocks
         self.published = 0      # number of full blocks published
+        self.serial = next(_SERIAL)   # tells sequences apart, also those of one request
+
+    def fork(self, count: int) -> Tuple["SequenceState", Optional[Tuple[int, int, int]]]:
+        """A sequence of its own that begins with the first `count` tokens of this one and has the
+        keys of all but the last of them: it shares the blocks that are full before that token, and
+        has a copy of the block that the token lies in, which it writes into. Returns it, and that
+        copy as (source, target, tokens) for PagedKVCache.copy_blocks, None where nothing is copied.
+        The copy has to be made before either sequence writes keys again."""
+        if self.state_pool is not None:
+            raise ValueError("recurrent state does not fork")
+        if not 0 < count <= min(len(self.token_ids), self.num_cached + 1):
+            raise ValueError(f"a fork at token {count} of {len(self.token_ids)}, {self.num_cached} with keys")
+        cache, bs = self.cache, self.cache.block_size
+        keep, used = divmod(count - 1, bs)
+        target = cache.alloc_block() if used else None
+        child = SequenceState(cache, self.token_ids[:count])
+        child.blocks = self.blocks[:keep]
+        for bid in child.blocks:
+            cache.retain(bid)
+        child.num_cached = count - 1
+        child.published = min(self.published, keep)
+        for i in range(child.published):
+            child.chain_h = cache.chain_hash(child.chain_h, child.token_ids[i * bs : (i + 1) * bs])
+        if target is None:
+            return child, None
+        child.blocks.append(target)
+        return child, (self.blocks[keep], target, used)
 
     def reuse_prefix(self) -> int:
         blocks, n = self.cache.lookup_prefix(self.token_ids)

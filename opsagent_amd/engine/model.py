@@ -67,6 +67,11 @@ class ForwardBatch:
     seq_lens: Optional[torch.Tensor] = None     # [B] int32
     decode_workspace: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
     nsplit: Optional[int] = None
+    # decode of rows that begin with the same cache blocks: leaders and shared blocks [B] int32
+    # (ops.attention_decode_shared), and the step's plan, made by the forward
+    leaders: Optional[torch.Tensor] = None
+    shared: Optional[torch.Tensor] = None
+    shared_plan: Optional[ops.SharedPlan] = None
     # kind == "mixed": a flat multi-sequence step (prompt portions beside
     # decoded tokens); geometry in an ops.mixer_ops.SeqBatch
     seq_batch: Optional[object] = None
@@ -152,7 +157,7 @@ class Attention(nn.Module):
         parts: bool = False,      # the output may be a product's parts (ops.linear_parts)
     ) -> torch.Tensor:
         T = x.shape[0]
-        fused = fb.kind == "decode" and x.is_cuda and _rope_attn_fused()
+        fused = fb.kind == "decode" and x.is_cuda and fb.leaders is None and _rope_attn_fused()
         qkv = self._qkv(x, fused)  # hipBLASLt / HIP gemv / fp8 at decode
         if isinstance(qkv, ops.PlaneSum):
             if fused:
@@ -205,6 +210,12 @@ class Attention(nn.Module):
                 k, v = k.unsqueeze(0), v.unsqueeze(0)
             out = ops.attention_prefill(
                 q.unsqueeze(0), k, v, scale=self.scale, steady=self.fp8, slots=slots,
+            )
+            out = out.view(T, self.hq * self.hd)
+        elif fb.leaders is not None:
+            out = ops.attention_decode_shared(
+                q, k_cache, v_cache, fb.block_table, fb.seq_lens, fb.leaders, fb.shared,
+                scale=self.scale, plan=fb.shared_plan,
             )
             out = out.view(T, self.hq * self.hd)
         else:
@@ -434,6 +445,7 @@ class LlamaForCausalLM(nn.Module):
         return (
             x.is_cuda
             and fb.kind == "decode"
+            and fb.leaders is None
             # fused-norm wins at B=1 (3.73 -> 3.61 ms/step) but its rstd
             # prologue scales with batch and measured a net loss at c=8
             and x.shape[0] <= int(os.environ.get("OPSAGENT_FUSED_DECODE_MAX_B", "1"))
@@ -474,6 +486,12 @@ class LlamaForCausalLM(nn.Module):
             torch.cuda.empty_cache()
 
     def forward(self, fb: ForwardBatch, kv_caches: List[Tuple[torch.Tensor, torch.Tensor]]):
+        if fb.leaders is not None and fb.shared_plan is None:
+            # the layers' lengths, blocks and heads are the same, and so is their plan
+            at, k_cache = self.layers[0].attn, kv_caches[0][0]
+            fb.shared_plan = ops.shared_decode_plan(
+                fb.seq_lens, fb.leaders, fb.shared, (at.hq, at.hk), at.hd,
+                fb.block_table.shape[1], k_cache.shape[1])
         if self._use_fused_decode(fb, fb.input_ids):
             residual = F.embedding(fb.input_ids, self.embed).contiguous()
             for i, layer in enumerate(self.layers):

@@ -239,7 +239,7 @@ class ChatCompletionAPI:
             stop=[stop] if isinstance(stop, str) else stop,
         )
         n = max(1, int(n))
-        futs = [self.loop.submit(prompt_ids, params) for _ in range(n)]
+        futs = self.loop.submit_choices(prompt_ids, params, n)
         results = [f.result() for f in futs]
         total = sum(len(ids) for ids, _ in results)
         return {
@@ -324,7 +324,7 @@ class ChatCompletionAPI:
         # concurrent callers (and the n>1 fan-out) batch together in the
         # engine loop's continuous batches
         n = max(1, int(n))
-        futs = [self.loop.submit(prompt_ids, params) for _ in range(n)]
+        futs = self.loop.submit_choices(prompt_ids, params, n)
         results = [f.result() for f in futs]
         lp_contents = [getattr(f, "logprob_content", None) for f in futs]
         perf.record_metric("engine_chat_ms", (time.perf_counter() - t0) * 1000.0)

@@ -74,9 +74,26 @@ class EngineLoop:
                 "TP follower ranks do not accept requests — submit to rank 0"
             )
         fut: Future = Future()
-        self._submit_q.put((list(prompt_ids), params or SamplingParams(), fut, None))
+        self._submit_q.put((list(prompt_ids), params or SamplingParams(), fut, None, None))
         self._wake.set()
         return fut
+
+    def submit_choices(self, prompt_ids: List[int], params: Optional[SamplingParams] = None,
+                       n: int = 1) -> List[Future]:
+        """n futures of one prompt. With the engine's fork_choices the prompt is read once, and the
+        others take over its keys."""
+        if not self.engine.fork_choices:
+            return [self.submit(prompt_ids, params) for _ in range(n)]
+        if self.is_follower:
+            raise RuntimeError(
+                "TP follower ranks do not accept requests — submit to rank 0"
+            )
+        futs = [Future() for _ in range(n)]
+        for fut in futs:
+            self._submit_q.put((list(prompt_ids), params or SamplingParams(), fut, None,
+                                None if fut is futs[0] else futs[0]))
+        self._wake.set()
+        return futs
 
     def generate(self, prompt_ids: List[int], params: Optional[SamplingParams] = None):
         return self.submit(prompt_ids, params).result()
@@ -86,7 +103,7 @@ class EngineLoop:
         future resolves to (output_ids, finish_reason) at completion."""
         tq: "queue.Queue" = queue.Queue()
         fut: Future = Future()
-        self._submit_q.put((list(prompt_ids), params or SamplingParams(), fut, tq))
+        self._submit_q.put((list(prompt_ids), params or SamplingParams(), fut, tq, None))
         self._wake.set()
 
         def _iter():
@@ -118,11 +135,13 @@ class EngineLoop:
     def _drain_submissions(self) -> None:
         while True:
             try:
-                ids, params, fut, tq = self._submit_q.get_nowait()
+                ids, params, fut, tq, first = self._submit_q.get_nowait()
             except queue.Empty:
                 return
             try:
-                rid = self.engine.add_request(ids, params)
+                rid = self.engine.add_request(ids, params) if first is None else (
+                    self.engine.add_request(ids, params, getattr(first, "request_id", None)))
+                fut.request_id = rid
                 if tq is not None:
                     self.engine.requests[rid].stream_queue = tq
                 self._futures[rid] = fut

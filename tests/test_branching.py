@@ -1,0 +1,358 @@
+"""Sequences that grow out of one prompt: forks of a cached sequence, the pool compacted and
+shrunk under running ones, decode steps that read common blocks once."""
+
+import itertools
+import random
+
+import pytest
+import torch
+
+from opsagent_amd.engine import engine as engine_module
+from opsagent_amd.engine.engine import LLMEngine, SamplingParams
+from opsagent_amd.engine.kv_cache import (
+    BlockAllocatorError,
+    PagedKVCache,
+    SequenceState,
+    StateSlotPool,
+    shared_prefixes,
+)
+from opsagent_amd.engine.serving import EngineLoop
+
+gpu = pytest.mark.gpu
+
+
+# -- which rows share ---------------------------------------------------------------------------
+def _saved(tables, full, groups):
+    total = 0
+    for rows in groups:
+        least = min(full[b] for b in rows)
+        same = 0
+        while same < least and len({tables[b][same] for b in rows}) == 1:
+            same += 1
+        total += (len(rows) - 1) * same
+    return total
+
+
+def _partitions(rows):
+    if not rows:
+        yield []
+        return
+    head, rest = rows[0], rows[1:]
+    for k in range(len(rest) + 1):
+        for mates in itertools.combinations(rest, k):
+            left = [r for r in rest if r not in mates]
+            for more in _partitions(left):
+                yield [[head, *mates], *more]
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_shared_prefixes_save_the_most(seed):
+    rng = random.Random(seed)
+    n = rng.randint(1, 6)
+    tables = []
+    for b in range(n):
+        if tables and rng.random() < 0.8:
+            old = rng.choice(tables)
+            keep = rng.randint(0, len(old))
+            tables.append(old[:keep] + [100 * b + i for i in range(rng.randint(0, 3))])
+        else:
+            tables.append([100 * b + i for i in range(rng.randint(0, 6))])
+    full = [max(0, len(t) - rng.randint(0, 1)) for t in tables]
+    leaders, shared, saved = shared_prefixes(tables, full)
+    best = max(_saved(tables, full, g) for g in _partitions(list(range(n))))
+    groups = {}
+    for b in range(n):
+        assert leaders[leaders[b]] == leaders[b]
+        assert tables[b][: shared[b]] == tables[leaders[b]][: shared[b]] and shared[b] <= full[b]
+        groups.setdefault(leaders[b], []).append(b)
+    assert saved == best == sum((len(g) - 1) * shared[g[0]] for g in groups.values())
+
+
+def test_shared_prefixes_of_nothing():
+    assert shared_prefixes([], []) == ([], [], 0)
+    assert shared_prefixes([[], []], [0, 0]) == ([0, 1], [0, 0], 0)
+
+
+# -- forks --------------------------------------------------------------------------------------
+def _cache(blocks=16, bs=4, **kw):
+    cache = PagedKVCache(2, 1, 8, bs, blocks, "cpu", torch.float32, **kw)
+    for k, v in cache.layers:
+        k.normal_()
+        v.normal_()
+    return cache
+
+
+def _sequence(cache, tokens):
+    seq = SequenceState(cache, tokens)
+    seq.ensure_capacity(len(tokens))
+    seq.num_cached = len(tokens)
+    seq.publish_full_blocks()
+    return seq
+
+
+@pytest.mark.parametrize("prefix_caching", [True, False])
+@pytest.mark.parametrize("count", [1, 2, 4, 5, 8, 9, 11])
+def test_fork(count, prefix_caching):
+    cache = _cache(prefix_caching=prefix_caching)
+    tokens = list(range(20, 31))
+    seq = _sequence(cache, tokens)
+    free = cache.num_free()
+    child, copy = seq.fork(count)
+    keep, used = divmod(count - 1, 4)
+    assert child.token_ids == tokens[:count] and child.num_cached == count - 1
+    assert child.blocks[:keep] == seq.blocks[:keep] and len(child.blocks) == keep + bool(used)
+    assert (copy is None) == (used == 0)
+    if copy:
+        assert copy == (seq.blocks[keep], child.blocks[keep], used)
+        assert child.blocks[keep] not in seq.blocks
+        cache.copy_blocks(*[[x] for x in copy])
+        for k, v in cache.layers:
+            for t in (k, v):
+                assert torch.equal(t[copy[1], :used], t[copy[0], :used])
+                assert not torch.equal(t[copy[1], used:], t[copy[0], used:])
+    # it goes on by itself, and publishes what is new
+    child.token_ids += [5, 6, 7, 8, 9]
+    child.ensure_capacity(len(child.token_ids))
+    child.num_cached = len(child.token_ids)
+    child.publish_full_blocks()
+    assert len(set(child.blocks)) == len(child.blocks)
+    child.free()
+    seq.free()
+    assert cache.num_free() == 16 and free < 16
+    again = SequenceState(cache, tokens + [1])
+    assert again.reuse_prefix() == (8 if prefix_caching else 0)
+
+
+def test_fork_gives_the_same_hash_chain():
+    cache = _cache()
+    seq = _sequence(cache, list(range(13)))
+    child, _ = seq.fork(13)
+    twin = SequenceState(cache, list(range(13)))
+    twin.reuse_prefix()
+    assert (child.chain_h, child.published, child.blocks[:3]) == (twin.chain_h, twin.published, twin.blocks)
+
+
+def test_forks_refused():
+    cache = _cache(blocks=3)
+    seq = _sequence(cache, list(range(10)))
+    for count in (0, -1, 11):
+        with pytest.raises(ValueError, match="fork at token"):
+            seq.fork(count)
+    refs = list(cache._ref)
+    with pytest.raises(BlockAllocatorError):
+        seq.fork(10)
+    assert cache._ref == refs
+    pool = StateSlotPool(2, [{"s": (2,)}], "cpu")
+    with pytest.raises(ValueError, match="state"):
+        SequenceState(cache, [1], pool).fork(1)
+
+
+# -- the pool compacted and shrunk --------------------------------------------------------------
+def _contents(cache, seqs):
+    return [[t[b].clone() for b in s.blocks for t in (k, v)] for s in seqs for k, v in cache.layers]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for xs, ys in zip(a, b) for x, y in zip(xs, ys))
+
+
+@pytest.mark.parametrize("shrink", [False, True])
+@pytest.mark.parametrize("shapes", [None, [(2, 8, 8), None, (1, 8, 4, "prefix"), (2, 8, 6, "vheads", 1)]])
+def test_compact(shrink, shapes):
+    cache = PagedKVCache(4, 1, 8, 4, 24, "cpu", torch.float32, layer_shapes=shapes)
+    for k, v in cache.layers:
+        if k is not None:
+            k.normal_()
+            if v.data_ptr() != k.data_ptr():
+                v.normal_()
+    cache.layers = [kv for kv in cache.layers if kv[0] is not None] if not shrink else cache.layers
+    seqs = [_sequence(cache, [100 * i + j for j in range(4 + 3 * i)]) for i in range(5)]
+    shared = SequenceState(cache, seqs[4].token_ids + [3])
+    shared.reuse_prefix()
+    seqs[0].free()                             # its block stays cached, the oldest
+    seqs[2].free()
+    live = [seqs[1], seqs[3], seqs[4], shared]
+    layers = [kv for kv in cache.layers if kv[0] is not None]
+    before = [[t[b].clone() for b in s.blocks for t in kv] for s in live for kv in layers]
+    cached = [i for i, s in ((0, seqs[0]), (2, seqs[2]))]
+    if shrink:
+        used = len({b for s in live for b in s.blocks})
+        cache.shrink(used + 1, live)           # room for one of the cached blocks
+        assert cache.num_blocks == used + 1 and cache.num_free() == 1
+        assert all(t.shape[0] == used + 1 for kv in cache.layers for t in kv if t is not None)
+    else:
+        n = cache.compact(live)
+        assert sorted(cache._free) == list(range(n, 24))
+        assert max(b for s in live for b in s.blocks) < n
+    layers = [kv for kv in cache.layers if kv[0] is not None]
+    after = [[t[b] for b in s.blocks for t in kv] for s in live for kv in layers]
+    assert _same(before, after)
+    assert shared.blocks[: len(seqs[4].blocks) - 1] == seqs[4].blocks[:-1]
+    # the prefix cache still finds what it held (the newest of it where there was room for one)
+    found = {i: SequenceState(cache, [100 * i + j for j in range(4 + 3 * i)] + [7]) for i in cached}
+    hits = {i: s.reuse_prefix() for i, s in found.items()}
+    assert hits == ({0: 4, 2: 8} if not shrink else {0: 0, 2: 0}) or shrink
+    for s in [*live, *found.values()]:
+        s.free()
+    assert cache.num_free() == cache.num_blocks and not any(cache._ref)
+    while cache.num_free():
+        cache.alloc_block()
+    with pytest.raises(BlockAllocatorError):
+        cache.alloc_block()
+
+
+def test_compact_takes_every_sequence():
+    cache = _cache()
+    a, b = _sequence(cache, list(range(6))), _sequence(cache, list(range(50, 60)))
+    with pytest.raises(ValueError, match="every sequence"):
+        cache.compact([a])
+    with pytest.raises(ValueError, match="every sequence"):
+        cache.compact([a, b, b])
+    with pytest.raises(BlockAllocatorError, match="in use"):
+        cache.shrink(4, [a, b])
+    for blocks in (0, 17):
+        with pytest.raises(ValueError, match="does not shrink"):
+            cache.shrink(blocks, [a, b])
+    assert cache.compact([a, b]) == 5
+
+
+def test_drop_cached():
+    cache = _cache()
+    seqs = [_sequence(cache, [10 * i + j for j in range(4)]) for i in range(3)]
+    for s in seqs:
+        s.free()
+    assert cache.drop_cached(2) == 1 and cache.num_free() == 16
+    assert [SequenceState(cache, [10 * i + j for j in range(5)]).reuse_prefix() for i in range(3)] == [0, 4, 4]
+    assert cache.drop_cached() == 0
+
+
+# -- engines ------------------------------------------------------------------------------------
+def _engine(**kw):
+    cfg = dict(model="llama3-tiny", max_batch_size=8, kv_block_size=4, max_seq_len=128, spec_decode=False)
+    if torch.cuda.is_available():
+        cfg.update(model="llama3-micro", kv_block_size=32, max_seq_len=1024, kv_num_blocks=300)
+    return LLMEngine({**cfg, **kw})
+
+
+def _drain(eng, ids):
+    for _ in range(600):
+        if all(eng.requests[i].finished for i in ids):
+            return [eng.requests.pop(i).output_ids for i in ids]
+        eng.step()
+    raise AssertionError("not done in 600 steps")
+
+
+PARAMS = SamplingParams(max_new_tokens=9, stop_on_eos=False)
+
+
+@pytest.mark.parametrize("length", [1, 4, 5, 8, 30])
+def test_choices_fork(length):
+    """n choices of a prompt: one prefill, and what separate requests answer."""
+    prompt = [(7 * i) % 250 for i in range(length)]
+    plain = _engine(prefix_caching=True)
+    want = _drain(plain, [plain.add_request(prompt, PARAMS)])[0]
+    eng = _engine(fork_choices=True)
+    prefilled = []
+    chunk = eng._prefill_chunk
+    eng._prefill_chunk = lambda r: (prefilled.append(r.req_id), chunk(r))
+    first = eng.add_request(prompt, PARAMS)
+    ids = [first] + [eng.add_request(prompt, PARAMS, fork_of=first) for _ in range(3)]
+    other = eng.add_request([9] * 6, PARAMS)              # is not held up by those that wait
+    got = _drain(eng, ids + [other])
+    assert set(prefilled) == {first, other}
+    if not torch.cuda.is_available():                     # the same arithmetic in every batch
+        assert all(g == want for g in got[:4])
+    assert all(len(g) == 9 for g in got) and got[1] == got[2] == got[3]
+    assert not any(eng.kv._ref) and eng.kv.num_free() == eng.kv.num_blocks
+
+
+def test_a_fork_of_something_else_is_prefilled():
+    eng = _engine(fork_choices=True)
+    first = eng.add_request([1, 2, 3, 4, 5], PARAMS)
+    ids = [first, eng.add_request([1, 2, 3, 9, 5], PARAMS, fork_of=first), eng.add_request([4, 4], PARAMS, fork_of=99)]
+    plain = _engine()
+    want = [_drain(plain, [plain.add_request(p, PARAMS)])[0] for p in ([1, 2, 3, 4, 5], [1, 2, 3, 9, 5], [4, 4])]
+    got = _drain(eng, ids)
+    assert got == want or torch.cuda.is_available()
+
+
+def test_a_fork_of_an_ended_request():
+    eng = _engine(fork_choices=True)
+    first = eng.add_request([1, 2, 3, 4, 5], PARAMS)
+    want = _drain(eng, [first])
+    assert _drain(eng, [eng.add_request([1, 2, 3, 4, 5], PARAMS, fork_of=first)]) == want or torch.cuda.is_available()
+
+
+def test_forks_under_cache_pressure():
+    """Fewer blocks than the choices need: some wait or are preempted, all of them end."""
+    eng = _engine(fork_choices=True, kv_num_blocks=14 if not torch.cuda.is_available() else 6)
+    prompt = [(3 * i) % 250 for i in range(eng.block_size * 2 + 1)]
+    params = SamplingParams(max_new_tokens=3 * eng.block_size, stop_on_eos=False)
+    first = eng.add_request(prompt, params)
+    ids = [first] + [eng.add_request(prompt, params, fork_of=first) for _ in range(3)]
+    got = _drain(eng, ids)
+    assert all(g for g in got) and not any(eng.kv._ref)
+
+
+def test_the_loop_forks_choices():
+    eng = _engine(fork_choices=True)
+    loop = EngineLoop(eng)
+    try:
+        futs = loop.submit_choices([5, 6, 7, 8, 9, 10], PARAMS, 3)
+        got = [f.result(timeout=60)[0] for f in futs]
+        assert got[1] == got[2] and all(len(g) == 9 for g in got)
+        assert loop.submit_choices([5, 6], PARAMS, 1)[0].result(timeout=60)
+    finally:
+        loop.shutdown()
+
+
+@pytest.mark.parametrize("hipgraph", [False, True])
+def test_shared_prefix_steps(hipgraph, monkeypatch):
+    """Steps that read common blocks once answer what the others do."""
+    monkeypatch.setattr(engine_module, "SHARED_LEAST", 1)
+    on_gpu = torch.cuda.is_available()
+    system = [(11 * i) % 250 for i in range(40 if not on_gpu else 200)]
+    prompts = [system + [i, 3 * i + 1] for i in range(4)] + [[8, 7, 6]] + [system[:21] + [2]]
+    runs = []
+    for shared in (False, True):
+        eng = _engine(shared_prefix=shared, use_hipgraph=hipgraph)
+        steps = []
+        if shared:
+            find = eng._find_shared
+            eng._find_shared = lambda batch: (steps.append(find(batch)), steps[-1])[1]
+        seen = []
+        sample = eng._sample_and_append
+        eng._sample_and_append = lambda batch, logits: (
+            seen.append({r.req_id: logits[i].float().cpu() for i, r in enumerate(batch)}), sample(batch, logits))
+        out = _drain(eng, [eng.add_request(p, PARAMS) for p in prompts])
+        runs.append((out, seen))
+        assert not shared or any(steps)
+    (want, logits), (got, shared_logits) = runs
+    if not on_gpu:
+        assert got == want
+    # the first decoded tokens follow the same prefills: attention differs by roundings to bfloat16,
+    # a few 2^-8 in each of four layers
+    first = [s for s in shared_logits if len(s) == len(prompts)][0]
+    plain = [s for s in logits if len(s) == len(prompts)][0]
+    for rid, row in plain.items():
+        assert (first[rid] - row).norm() <= 2.0 ** -4 * row.norm()
+
+
+def test_shrinks_between_steps(monkeypatch):
+    monkeypatch.setattr(engine_module, "SHARED_LEAST", 1)
+    prompts = [[(5 * i + k) % 250 for i in range(30)] for k in range(3)]
+    outs = []
+    for shrink in (False, True):
+        eng = _engine(shared_prefix=True, fork_choices=True)
+        done = eng.add_request([9] * 40, SamplingParams(max_new_tokens=2, stop_on_eos=False))
+        _drain(eng, [done])                               # leaves blocks in front of the others
+        ids = [eng.add_request(p, PARAMS) for p in prompts]
+        ids.append(eng.add_request(prompts[0], PARAMS, fork_of=ids[0]))
+        for _ in range(6):
+            eng.step()
+        if shrink:
+            live = {b for r in eng.running for b in r.seq.blocks}
+            eng.shrink_cache(len(live) + 16)
+            assert eng.kv.num_blocks == len(live) + 16
+        outs.append(_drain(eng, ids))
+    assert outs[0] == outs[1]
