@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t sh_pack(float lo, float hi) {
 }
 
 // ---- plan --------------------------------------------------------------------------------------
-// PLAN, in ints: items (padded to 8) | first[B] | splits[B] | members[B], rows group after group |
+// PLAN, in ints: items, sizes of the line (padded to 8) | first[B] | splits[B] | members[B], rows group after group |
 // units of 8: table row (-1: none), first key, end, place of the group's tile in members, members of
 // the tile (0: the table row alone), split, next unit of the item (-1: none), the table row's first slot.
 //
@@ -203,7 +203,10 @@ __global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restr
             }
             s += __builtin_amdgcn_readlane(is, WAVE - 1);
         }
-        if (lane == 0) plan[0] = min(items, z.max_units);
+        if (lane == 0) {
+            plan[0] = min(items, z.max_units);
+            plan[1] = (int)behind;
+        }
     }
     __syncthreads();
     auto write = [&](int u, int row, int k0, int k1, int place, int n, int split, int next) {
@@ -279,6 +282,11 @@ struct SharedArgs {
     int B, Hq, Hk, G, pages, shift, slots;
     float scale;                                                                 // times log2(e)
     PlanSizes z;
+    // Whether the rows' own keys are more than stays in the last cache until the next step, half of its
+    // 256 MB: then they are read without being kept. 48 rows of up to 2000 tokens (197 MB) 50.4 -> 42.5
+    // us, 64 of up to 512 (67 MB) 20.1 -> 21.2.
+    int64_t size_bytes;                                                          // of 64 keys and values
+    __device__ bool much(int sizes) const { return sizes * size_bytes >= (int64_t)128 << 20; }
 };
 
 constexpr int IDS = 1024;                          // pages of a unit that lie in LDS at a time
@@ -289,7 +297,8 @@ struct SharedPlaces {
     int ids[IDS], rows[TILE], slots[TILE];
 };
 struct OwnPlan {
-    int4 first[2];                                 // row (-1: none), first key, end, members | slot, next row, items
+    int4 first[2];                                 // row (-1: none), first key, end, members |
+                                                   // slot, next row, items, sizes of the line
     int4 row[WAVE];                                // first key, end, slot, next row
     int count[WAVE], common[WAVE];
 };
@@ -298,7 +307,9 @@ struct OwnPlan {
 // takes a microsecond of every block, and a launch before this one 10 (with its wait for the chip).
 __device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan& own, SharedPlaces& places) {
     const PlanSizes& z = a.z;
-    const int lane = threadIdx.x & (WAVE - 1), B = z.B;
+    int lane = threadIdx.x & (WAVE - 1);
+    asm volatile("" : "+v"(lane));                           // nothing of this is kept meanwhile
+    const int B = z.B;
     const bool in = lane < B;
     const int most = (int)min((int64_t)z.width << z.shift, (int64_t)INT32_MAX - 4096);
     const int keys = in ? min(max(a.seq_lens[lane], 0), most) : 0;
@@ -348,7 +359,7 @@ __device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan
     const int start = p + (from < upto ? cut(from) : rest), start_link = from < upto ? -1 : link;
     own.row[lane] = int4{p, start, slot + shared_chunks, start_link};
     if (lane == 0) own.first[0] = int4{-1, 0, 0, 0};
-    if (lane == 0) own.first[1] = int4{0, -1, ahead + lines, 0};
+    if (lane == 0) own.first[1] = int4{0, -1, ahead + lines, (int)behind};
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (item < ahead) {
         const int lead = __builtin_ctzll(__ballot(unit_of <= item && item < unit_of + nu));
@@ -367,16 +378,17 @@ __device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan
         const int i = item - ahead;
         if (rest > 0 && i == from - 1 && before < from) {
             own.first[0] = int4{lane, p, start, 0};
-            own.first[1] = int4{slot + shared_chunks, start_link, ahead + lines, 0};
+            own.first[1] = int4{slot + shared_chunks, start_link, ahead + lines, (int)behind};
         } else if (rest > 0 && i >= from && i < upto) {
             own.first[0] = int4{lane, p + cut(i), p + (i + 1 < upto ? cut(i + 1) : rest), 0};
-            own.first[1] = int4{slot + shared_chunks + 1 + i - from, i + 1 < upto ? -1 : link, ahead + lines, 0};
+            own.first[1] = int4{slot + shared_chunks + 1 + i - from, i + 1 < upto ? -1 : link, ahead + lines, (int)behind};
         }
     }
 }
 
 struct SharedUnit {
     int row, begin, end, group, slot, columns;     // group: members, their rows and slots in LDS
+    bool once;                                     // keys that no cache holds until the next step
 };
 // Four waves take a unit's chunk for one key head. A wave has up to 32 columns (MT tiles of 16), so
 // KG groups of waves share the keys out, 32 in turn, and the 4 / KG waves of a group the columns:
@@ -507,7 +519,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             for (int p = 0; p < 32 / RPP; ++p) {
                 int at;
                 const int place = place_of(p, at);
-                lds_transfer16(to + p * 1024, __umul24(at, token) + place, rows);
+                if (KG == 4 && unit.once) lds_transfer16<true>(to + p * 1024, __umul24(at, token) + place, rows);
+                else lds_transfer16(to + p * 1024, __umul24(at, token) + place, rows);
             }
         } else {
 #pragma unroll
@@ -724,9 +737,10 @@ __global__ __launch_bounds__(256, 2) void shared_attn_kernel(SharedArgs a) {
         const int* const members = first + 2 * a.B;
         const int4* const units = reinterpret_cast<const int4*>(a.plan + plan_units(a.B));
         // the number of items and the first one's record in one wait: there is room for `runs` of them
-        const int count = a.plan[0];
+        const int count = a.plan[0], behind = a.plan[1];
         int4 x = units[2 * (size_t)begin], y = units[2 * (size_t)begin + 1];
         const int items = same(count);
+        const bool once = a.much(same(behind));
         for (int i = begin; i < items; i += a.z.runs)
             for (int u = i; u >= 0;) {
                 if (u != begin) {
@@ -734,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void shared_attn_kernel(SharedArgs a) {
                     y = units[2 * (size_t)u + 1];
                 }
                 const int place = same(x.w), split = same(y.y);
-                SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(y.x), same(y.w) + split, 0};
+                SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(y.x), same(y.w) + split, 0, !same(y.x) && once};
                 unit.columns = max(unit.group, 1) * a.G;
                 u = same(y.z);
                 if ((uint32_t)unit.row >= (uint32_t)a.B) continue;   // an item without units
@@ -753,13 +767,14 @@ __global__ __launch_bounds__(256, 2) void shared_attn_kernel(SharedArgs a) {
             int4 x = own.first[0];
             const int4 y = own.first[1];
             const int items = same(y.z);
-            SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(x.w), same(y.x), 0};
+            const bool once = a.much(same(y.w));
+            SharedUnit unit = {same(x.x), same(x.y), same(x.z), same(x.w), same(y.x), 0, !same(x.w) && once};
             unit.columns = max(unit.group, 1) * a.G;
             for (int next = same(y.y); (uint32_t)unit.row < (uint32_t)a.B;) {
                 take(unit);
                 if (next < 0) break;
                 x = own.row[next];
-                unit = SharedUnit{next, same(x.x), same(x.y), 0, same(x.z), a.G};
+                unit = SharedUnit{next, same(x.x), same(x.y), 0, same(x.z), a.G, once};
                 next = same(x.w);
             }
             if (i + a.z.runs >= items) break;
@@ -942,6 +957,7 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     a.shared = (const int*)shared;
     a.plan = (int*)plan;
     a.z = z;
+    a.size_bytes = (int64_t)64 * 2 * Hk * D * 2;
     a.o_part = (float*)scratch;
     a.ml_part = a.o_part + (size_t)z.max_slots * Hq * D;
     int64_t* const steps[8] = {&a.q_row, &a.q_head, &a.k_page, &a.k_token, &a.k_head, &a.v_page, &a.v_token, &a.v_head};

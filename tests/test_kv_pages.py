@@ -101,6 +101,7 @@ def test_pages_apart():
 
 
 @gpu
+@torch.inference_mode()      # as the engine captures: one kind of capture for a process
 def test_captured():
     layers = _layers("cuda", [(2, 64)] * 2)
     table = ops.KVPages(layers)

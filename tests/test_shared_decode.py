@@ -270,6 +270,7 @@ def test_a_plan_is_made_once_for_all_layers():
 
 
 @gpu
+@torch.inference_mode()      # as the engine captures: one kind of capture for a process
 def test_captured_steps_follow_lengths_and_leaders():
     """Two graphs over one set of buffers, replayed in turn with other lengths, groups and eager
     work between."""
