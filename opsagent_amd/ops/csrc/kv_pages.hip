@@ -23,16 +23,21 @@ struct PageCopies {                        // source i goes to dst[begin[i]] .. 
 };
 static_assert(sizeof(PageTensors) + sizeof(PageCopies) + 32 <= 4096, "what a launch may carry");
 
-// Grid: 4-KiB slices of a page, tensors, sources.
+// Grid: 4-KiB slices of a page, sources, tensors: the copies of a tensor side by side, and 16 bytes a
+// thread. What is written is not kept: it is more than the next reader's share of a cache where it
+// takes time at all. us, by size: 96 pages of 64 KiB in 64 tensors (805 MB in and out) 128 (6.3 TB/s;
+// kept 135, tensors side by side 157, 64 bytes a thread 162), three copies of 16 pages' first tokens in
+// 160 tensors (291 MB) 66 (77, 78, 99), three of one in 64 4, with the launch.
 __global__ __launch_bounds__(256) void kv_pages_copy_kernel(PageTensors tensors, PageCopies copies,
                                                             int64_t step, int row) {
-    char* const base = tensors.base[blockIdx.y];
-    const int c = blockIdx.z;
+    typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+    char* const base = tensors.base[blockIdx.z];
+    const int c = blockIdx.y;
     const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
     if (at >= (int64_t)copies.tokens[c] * row) return;
-    const uint4 piece = *reinterpret_cast<const uint4*>(base + copies.src[c] * step + at);
+    const u4 piece = *reinterpret_cast<const u4*>(base + copies.src[c] * step + at);
     for (int i = copies.begin[c]; i < copies.begin[c + 1]; ++i)
-        *reinterpret_cast<uint4*>(base + copies.dst[i] * step + at) = piece;
+        __builtin_nontemporal_store(piece, reinterpret_cast<u4*>(base + copies.dst[i] * step + at));
 }
 
 // bases: `tensors` addresses on the host, each of `pages` pages `step` bytes apart, a page `block`
@@ -68,7 +73,7 @@ extern "C" int oa_kv_pages_copy(void* stream, const uint64_t* bases, int tensors
             }
             c.begin[sources] = (uint16_t)nc;
             if (!most) continue;
-            hipLaunchKernelGGL(kv_pages_copy_kernel, dim3((unsigned)CEIL_DIV((int64_t)most * row, 4096), nt, sources),
+            hipLaunchKernelGGL(kv_pages_copy_kernel, dim3((unsigned)CEIL_DIV((int64_t)most * row, 4096), sources, nt),
                                dim3(256), 0, (hipStream_t)stream, t, c, step, row);
             HIP_CHECK_LAUNCH();
         }
