@@ -6,6 +6,12 @@ below its normal range, off by 2^-25 of the row's largest weight each; and 2^-12
 for float32 scores (128 products of at most 12 in all, to 2^-24 each of the partial sums, and
 as much again for the exponential)."""
 
+import ctypes
+import os
+import re
+import shutil
+import subprocess
+
 import pytest
 import torch
 
@@ -61,14 +67,14 @@ def _exact(c, scale=None):
         if n <= 0:
             continue
         pages = c["block_table"][b, : -(-n // bs)].long().cpu()
-        kk = k[pages].reshape(-1, Hk, D)[:n].repeat_interleave(Hq // Hk, 1)
-        vv = v[pages].reshape(-1, Hk, D)[:n].repeat_interleave(Hq // Hk, 1)
-        s = torch.einsum("hd,jhd->hj", q[b], kk) * scale
+        kk = k[pages].reshape(-1, Hk, D)[:n].transpose(0, 1).contiguous()      # [Hk, n, D]
+        vv = v[pages].reshape(-1, Hk, D)[:n].transpose(0, 1).contiguous()
+        s = q[b].view(Hk, Hq // Hk, D) @ kk.transpose(1, 2) * scale
         w = (s - s.amax(-1, keepdim=True)).exp()
         p = w / w.sum(-1, keepdim=True)
-        out[b] = torch.einsum("hj,jhd->hd", p, vv)
-        size = torch.einsum("hj,jhd->hd", p, vv.abs())
-        small = vv.abs().sum(0) / w.sum(-1)[:, None] * 2.0 ** -25
+        out[b] = (p @ vv).view(Hq, D)
+        size = (p @ vv.abs()).view(Hq, D)
+        small = (vv.abs().sum(1, keepdim=True) / w.sum(-1, keepdim=True) * 2.0 ** -25).view(Hq, D)
         tol[b] = h * (1 + h) * out[b].abs() + (h + 2.0 ** -12) * size
         if c["q"].dtype == torch.float16:
             tol[b] += small
@@ -246,6 +252,45 @@ def test_offsets_past_32_bits():
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hk,rows", [
+    (64, 64, [(0, 0, 9000)]),                             # keys shared out by the waves
+    (2560, 64, [(0, 0, 9000)]),                           # columns shared out
+    (64, 64, [(0, 9000, 9100), (0, 9000, 9001)]),
+])
+def test_more_pages_than_a_unit_lists(Hq, Hk, rows):
+    """Pages of one token, and more than 1024 of them in the keys that a block takes."""
+    c = _case(rows, Hq, Hk, 64, 1, seed=21)
+    _check(ops.attention_decode_shared(**c), c)
+
+
+@gpu
+def test_more_keys_than_a_cache_holds():
+    """Beyond 128 MB of them the rows' own keys are read in another way."""
+    c = _case([(0, 10, 320 + 1900 + i) for i in range(12)] + [(i, 0, 2000 + i) for i in range(12, 18)],
+              Hq=16, Hk=8, seed=22)
+    _check(ops.attention_decode_shared(**c), c)
+    plan = ops.shared_decode_plan(c["seq_lens"], c["leaders"], c["shared"], (16, 8), 128,
+                                  c["block_table"].shape[1], 32)
+    _check(ops.attention_decode_shared(**c, plan=plan), c)
+
+
+@gpu
+def test_calls_on_two_streams():
+    """Calls of different batches under way together share nothing."""
+    cases = [_case(GROUPS["long"], Hq=32, Hk=8, seed=23), _case(GROUPS["many rows"], seed=24)]
+    want = [ops.attention_decode_shared(**c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.attention_decode_shared(**c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+@gpu
 def test_equals_the_paged_form_and_itself():
     c = _case(GROUPS["long"], Hq=32, Hk=8, seed=14)
     got = ops.attention_decode_shared(**c)
@@ -395,3 +440,69 @@ def test_plain_form(name):
         c["block_table"][live].clamp(min=0), c["seq_lens"][live], None)
     assert torch.allclose(got[live], paged, atol=1e-5)
     assert ops.shared_decode_plan(c["seq_lens"], c["leaders"], c["shared"], (4, 2), 16, 9, 32) is None
+
+
+# -- the library ---------------------------------------------------------------------------------
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="no hipcc")
+@pytest.mark.parametrize("name", ["attention_shared.hip", "kv_pages.hip"])
+def test_kernels_use_no_scratch(name, tmp_path):
+    """Scratch reads would wait for every transfer that is under way."""
+    from opsagent_amd.ops import build
+
+    done = subprocess.run(
+        [build.HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", *build.HIP_FLAGS, "-c",
+         "-Rpass-analysis=kernel-resource-usage", os.path.join(build.CSRC, name), "-o",
+         str(tmp_path / "x.o")], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+    scratch = re.findall(r"ScratchSize \[bytes/lane\]: (\d+)", done.stderr)
+    assert scratch and set(scratch) == {"0"}
+
+
+def test_entry_points():
+    lib = os.path.join(os.path.dirname(ops.__file__), "libopsagent_kernels.so")
+    if not os.path.exists(lib):
+        pytest.skip("kernel library not built")
+    for name in ("oa_shared_plan_size", "oa_shared_plan", "oa_attention_decode_shared", "oa_kv_pages_copy"):
+        assert hasattr(ctypes.CDLL(lib), name), name
+
+
+def test_entries_check_what_they_are_given():
+    """Sizes that no launch takes, and pointers that it would not read right, come back as errors
+    before anything is launched."""
+    path = os.path.join(os.path.dirname(ops.__file__), "libopsagent_kernels.so")
+    if not os.path.exists(path):
+        pytest.skip("kernel library not built")
+    from opsagent_amd.ops import hip_lib
+
+    lib = ctypes.CDLL(path)
+    hip_lib._declare(lib)
+    ints, slots = ctypes.c_int(), ctypes.c_int()
+    size = lambda *s: lib.oa_shared_plan_size(*s, ctypes.byref(ints), ctypes.byref(slots))  # noqa: E731
+    assert size(4, 32, 8, 128) == 0 and ints.value > 0 and slots.value > 0
+    for bad in [(0, 32, 8, 128), (2049, 32, 8, 128), (4, 32, 0, 128), (4, 30, 8, 128), (4, 32, 8, 96),
+                (4, 129, 1, 64), (4, 4100, 4100, 64)]:
+        assert size(*bad) == -100, bad
+    good = [4096, 128, 262144, 1024, 128, 262144, 1024, 128, 9, 4, 32, 8, 128, 9, 50, 32, 0]
+    call = lambda n, q=16, scratch=16: lib.oa_attention_decode_shared(  # noqa: E731
+        None, q, 16, 16, 16, None, None, None, 16, scratch, 16, (ctypes.c_int64 * 17)(*n), 0.1)
+    for at, value, rc in [(9, 0, -100), (9, -1, -100), (13, 0, -100), (14, 0, -100), (14, 2 ** 31, -100),
+                          (15, 24, -101), (15, 0, -101), (0, 4092, -103), (4, 4, -103), (3, 2 ** 23, -105),
+                          (6, -8, -105)]:
+        n = list(good)
+        n[at] = value
+        assert call(n) == rc, (at, value)
+    assert call(good, q=8) == -103 and call(good, scratch=20) == -103
+    assert lib.oa_shared_plan(None, 16, 16, 16, 8, 4, 32, 8, 128, 9, 32) == -103
+    assert lib.oa_shared_plan(None, 16, 16, 16, 16, 4, 32, 8, 128, 0, 32) == -100
+    assert lib.oa_shared_plan(None, 16, 16, 16, 16, 4, 32, 8, 128, 9, 33) == -101
+    bases = (ctypes.c_uint64 * 1)(4096)
+    copy = lambda b, step, row, block, pages, c: lib.oa_kv_pages_copy(  # noqa: E731
+        None, b, 1, step, row, block, pages, (ctypes.c_int * 3)(*c), 1)
+    assert copy(bases, 512, 24, 8, 4, (0, 1, 8)) == -100
+    assert copy(bases, 520, 32, 8, 4, (0, 1, 8)) == -100
+    assert copy(bases, 512, 32, 0, 4, (0, 1, 8)) == -100
+    assert copy(bases, 512, 2 ** 20, 2 ** 12, 4, (0, 1, 8)) == -101
+    assert copy((ctypes.c_uint64 * 1)(4100), 512, 32, 8, 4, (0, 1, 8)) == -103
+    for c in [(-1, 1, 8), (4, 1, 8), (0, -1, 8), (0, 4, 8), (0, 1, 9), (0, 1, -1)]:
+        assert copy(bases, 512, 32, 8, 4, c) == -104
+    assert copy(bases, 512, 32, 8, 4, (0, 1, 0)) == 0        # nothing to copy: nothing is launched
