@@ -673,6 +673,22 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     __syncthreads();
     }
 
+    if constexpr (KG == 1) {                                 // a column's sums are one wave's
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int c = cg * 32 + m * 16 + col;
+            if (c >= columns) continue;
+            const int slot = unit.group ? places.slots[c / G] : unit.slot;
+            if (slot >= a.slots) continue;
+            const size_t to = (size_t)slot * a.Hq + h * G + c % G;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<sh_f4*>(a.o_part + to * D + d * 16 + g * 4) = o[m][d];
+            if (g == 0)
+                *reinterpret_cast<float2*>(a.ml_part + to * 2) =
+                    float2{mx[m] == -INFINITY ? -INFINITY : mx[m] * scale, sum[m][0]};
+        }
+        return;
+    }
     // a common maximum of the groups' sums of each column, in units of the weights' exponent
     __syncthreads();
     constexpr int PITCH = D + 4;
