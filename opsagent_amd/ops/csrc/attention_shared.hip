@@ -215,20 +215,23 @@ __global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restr
         d[0] = int4{row, k0, k1, place};
         d[1] = int4{n, split, next < z.max_units ? next : -1, row >= 0 ? slot_of[row] : 0};
     };
-    // a wave a group: its members in order, and its units
-    for (int b = wave; b < B; b += NW) {
-        const int p = common[b];
-        if (lead[b] != b || p <= 0) continue;
-        for (int b0 = 0, m = place[b]; b0 < B; b0 += WAVE) {
-            const bool mine = b0 + lane < B && lead[b0 + lane] == b;
-            const uint64_t all_mine = __ballot(mine);
-            if (mine) members[m + __builtin_popcountll(all_mine & ((1ull << lane) - 1))] = b0 + lane;
-            m += __builtin_popcountll(all_mine);
-        }
-        const int c = plan_chunk(p, per_run), tiles = (int)cdiv(count[b], z.tile);
-        for (int i = lane; i < chunks[b] * tiles; i += WAVE) {
-            const int part = i / tiles, from = i % tiles * z.tile;
-            write(unit_of[b] + i, b, part * c, min(part * c + c, p), place[b] + from, min(z.tile, count[b] - from), part, -1);
+    // a wave a group, in turn: its members in order, and its units
+    for (int r0 = 0, turn = 0; r0 < B; r0 += WAVE) {
+        uint64_t groups = __ballot(r0 + lane < B && lead[min(r0 + lane, B - 1)] == r0 + lane && common[min(r0 + lane, B - 1)] > 0);
+        for (; groups; groups &= groups - 1) {
+            if (turn++ % NW != wave) continue;
+            const int b = r0 + __builtin_ctzll(groups), p = common[b];
+            for (int b0 = 0, m = place[b]; b0 < B; b0 += WAVE) {
+                const bool mine = b0 + lane < B && lead[min(b0 + lane, B - 1)] == b;
+                const uint64_t all_mine = __ballot(mine);
+                if (mine) members[m + __builtin_popcountll(all_mine & ((1ull << lane) - 1))] = b0 + lane;
+                m += __builtin_popcountll(all_mine);
+            }
+            const int c = plan_chunk(p, per_run), tiles = (int)cdiv(count[b], z.tile);
+            for (int i = lane; i < chunks[b] * tiles; i += WAVE) {
+                const int part = i / tiles, from = i % tiles * z.tile;
+                write(unit_of[b] + i, b, part * c, min(part * c + c, p), place[b] + from, min(z.tile, count[b] - from), part, -1);
+            }
         }
     }
     // the unit behind a row's last one in its item: the next row's first, unless that begins an item
