@@ -1663,6 +1663,8 @@ class KVPages:
                 step = t.stride(0) * t.element_size() if t.shape[0] > 1 else row * self.block_size
                 if (row | step | t.data_ptr()) % 16:
                     raise ValueError("rows and pages of a cache on the GPU are multiples of 16 bytes")
+                if row * self.block_size >= 2 ** 31:
+                    raise ValueError(f"a cache page on the GPU is less than 2 GiB: got {row * self.block_size} bytes")
                 kinds.setdefault((step, row), []).append(t.data_ptr())
             for (step, row), at in kinds.items():
                 self._launches.append(((ctypes.c_uint64 * len(at))(*at), len(at), step, row))
@@ -1929,9 +1931,11 @@ def _shared_sizes(B: int, Hq: int, Hk: int, D: int) -> Tuple[int, int]:
 
 
 @functools.lru_cache(maxsize=1024)
-def _shared_table(width: int, block: int) -> None:
+def _shared_table(B: int, width: int, block: int) -> None:
     if block < 1 or block & (block - 1) or not 1 <= width < 2 ** 31:
         raise ValueError(f"a table of {width} pages of {block} tokens, which is no power of 2")
+    if B * width * block > 2 ** 35:
+        raise ValueError(f"tables of more than 2^35 tokens in all: {B} rows of {width} pages of {block}")
 
 
 def _int_rows(B: int, **rows: torch.Tensor) -> None:
@@ -1960,7 +1964,7 @@ def shared_decode_plan(
     if not seq_lens.device == leaders.device == shared.device:
         raise ValueError("seq_lens, leaders and shared are on one device")
     ints, _ = _shared_sizes(B, Hq, Hk, head_dim)
-    _shared_table(width, block_size)
+    _shared_table(B, width, block_size)
     lib, hip = _lib()
     with torch.cuda.device(seq_lens.device):
         plan = torch.empty(ints, dtype=torch.int32, device=seq_lens.device)
@@ -1991,7 +1995,7 @@ def _shared_geometry(qs, q_steps, q_dtype, ks, k_steps, k_dtype, vs, v_steps, v_
     if max(steps[3], steps[6]) >= 2 ** 23:
         raise ValueError("tokens of a page are less than 2^23 elements apart")
     ints, slots = _shared_sizes(B, Hq, Hk, D)
-    _shared_table(width, block)
+    _shared_table(B, width, block)
     sizes = (ctypes.c_int64 * 17)(*steps, t_steps[0] if B > 1 else 0, B, Hq, Hk, D, width, pages, block,
                                   q_dtype == torch.float16)
     return sizes, ints, slots * Hq * (D + 2), (B, Hq, Hk, D, width, block)

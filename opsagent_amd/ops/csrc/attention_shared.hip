@@ -9,8 +9,15 @@
 // of weights that they were taken with, and a second launch adds those up.
 //
 // Sums, maxima and weight sums are float32. Weights enter the product with the values as 16-bit
-// numbers of the cache's type, which is off by half a step of each weight and averages out over the
-// keys; the output is rounded to the same type.
+// numbers of the cache's type, as the matrix cores take them: off by half a step of each weight, which
+// averages out over the keys. Their sum is that of the rounded ones, so that what is divided by is what
+// was added up. The output is rounded to the same type.
+//
+// What bounds it (us; 32 heads on 8 and 64 on 8 of 128 channels, bfloat16): rows that share nothing, memory
+// (48 of up to 2000 tokens, 220 MB, 41: 5.4 TB/s); a few rows, latencies (a block's plan or its record 2
+// to 3, first keys 2, a step 1, sums 1; the second launch 3); many rows behind one prefix, matrix and
+// vector instructions of steps of 128 columns, 2.2 us for two blocks of a CU and 64 keys (128 rows
+// behind 16400 tokens 116 in all, 0.6 PFLOP/s).
 //
 //   q            [B, Hq, D] 16-bit, rows and heads any multiple of 8 elements apart
 //   kc, vc       [pages, 2^shift, Hk, D], pages, tokens and heads any multiple of 8 elements apart
@@ -59,6 +66,7 @@ constexpr int PLAN_HEAD = 8, UNIT = 8, UNIT_COST = 1;
 constexpr int PLAN_ROWS = 2048;
 constexpr int TILE = 128;                          // columns that a block takes
 constexpr int SIZES = 8;                           // sizes of an item that are looked at
+constexpr int64_t MOST_KEYS = (int64_t)1 << 35;    // that tables have room for: sizes and 8 of them are 32 bits
 
 struct PlanSizes {
     int B, G, width, shift, tile, runs, max_units, max_slots;    // tile: members of TILE columns
@@ -306,8 +314,8 @@ struct OwnPlan {
     int count[WAVE], common[WAVE];
 };
 
-// The plan of up to 64 rows, as shared_plan_kernel makes it, by one wave for itself: a lane a row. It
-// takes a microsecond of every block, and a launch before this one 10 (with its wait for the chip).
+// The plan of up to 64 rows, as shared_plan_kernel makes it, by one wave for itself: a lane a row. A
+// launch before this one takes longer, 8 us for 128 rows.
 __device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan& own, SharedPlaces& places) {
     const PlanSizes& z = a.z;
     int lane = threadIdx.x & (WAVE - 1);
@@ -491,7 +499,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     auto swz_v = [](int r) { return D == 128 ? r & 7 : (r >> 1) & 3; };
 
     // the unit's keys in spans whose pages lie in LDS; what a table should not hold reads the last page
-    const int span = (int)min((int64_t)(IDS - 16) << a.shift & ~(int64_t)127, (int64_t)INT32_MAX / 2);
+    const int span = (int)min((int64_t)(IDS - 16) << a.shift & ~(int64_t)127, (int64_t)1 << 30);
     int k0 = begin, k1 = begin + min(span, end - begin), page0 = k0 >> a.shift;
     auto place_pages = [&]() {
         const int* const table = a.block_table + row0 * a.table_row;
@@ -553,9 +561,18 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             }
         }
     };
-    auto weights = [&](int key) {
+    // values behind the chunk's last key are copies of its, and an infinite one times a weight of 0 would be
+    // no number. Waves that share a step all write the same zeros, each before it reads.
+    auto clear_behind = [&](char* vt, int key) {
+        int from = (int)threadIdx.x & (WAVE - 1);
+        asm volatile("" : "+v"(from));                       // nothing of this is kept meanwhile
+#pragma unroll 1
+        for (int at = (k1 - key) * ROW + from * 16; at < KEYS * ROW; at += 1024) *reinterpret_cast<uint4*>(vt + at) = uint4{0, 0, 0, 0};
+    };
+    auto weights = [&](int key, char* vt) {
         if (key + KEYS > k1) {
             asm volatile("" : : : "memory");                 // a branch: every other step goes without
+            if (KG < 4) clear_behind(vt, key);
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -604,17 +621,25 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
         v.p.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sh_s4*)hi);
         return v.u;
     };
+    // reads are three products ahead of their use: without a fixed order the compiler waits for each (128
+    // rows of 64 heads on 8 behind 16400 tokens 125 us; one ahead 117, two 118, three 116, four 121)
     auto add_values = [&](const char* vt) {
+        constexpr int AHEAD = 3, ALL = NJ / 2 * ND;
+        uint4 v[AHEAD];
 #pragma unroll
-        for (int half = 0; half < NJ / 2; ++half) {
+        for (int i = 0; i < AHEAD; ++i) v[i] = value(vt, i / ND, i % ND);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) sum[m] = sh_product<F16>(ones, pf[m][half], sum[m]);
+        for (int i = 0; i < ALL; ++i) {
+            const int half = i / ND, d = i % ND;
+            const uint4 now = v[i % AHEAD];
+            if (i + AHEAD < ALL) v[i % AHEAD] = value(vt, (i + AHEAD) / ND, (i + AHEAD) % ND);
+            if (d == 0)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const uint4 v = value(vt, half, d);
+                for (int m = 0; m < MT; ++m) sum[m] = sh_product<F16>(ones, pf[m][half], sum[m]);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) o[m][d] = sh_product<F16>(v, pf[m][half], o[m][d]);
-            }
+            for (int m = 0; m < MT; ++m) o[m][d] = sh_product<F16>(now, pf[m][half], o[m][d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -633,9 +658,12 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             wait_reads();
             const bool more = key + 128 < k1;
             if (more) load_rows(false, key + 128, ring_at);
-            weights(key);
+            weights(key, ring + PLANE);
             if (more) wait_transfers<PCS>();
-            else wait_transfers<0>();
+            else {
+                wait_transfers<0>();
+                if (key + KEYS > k1) clear_behind(ring + PLANE, key);
+            }
             add_values(ring + PLANE);
             wait_reads();
             if (more) load_rows(true, key + 128, ring_at + PLANE);
@@ -660,10 +688,10 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             wait_reads();
             asm volatile("s_barrier" : : : "memory");
             ask(i + 1);
-            const char* const at = ring + i % STAGES * STAGE;
+            char* const at = ring + i % STAGES * STAGE;
             if (busy && i < mine) {
                 products(at);
-                weights(key_of(i));
+                weights(key_of(i), at + PLANE);
                 add_values(at + PLANE);
             }
         }
@@ -936,6 +964,7 @@ extern "C" int oa_shared_plan(void* stream, const void* seq_lens, const void* le
     if (!shared_sizes(B, Hq, Hk, D) || width < 1) return -100;
     const int shift = shift_of(block_size);
     if (shift < 0) return -101;
+    if ((int64_t)B * width > MOST_KEYS >> shift) return -102;
     if ((uintptr_t)plan % 16 != 0) return -103;
     return launch_plan((hipStream_t)stream, seq_lens, leaders, shared, plan, plan_sizes(B, Hq, Hk, width, shift));
 }
@@ -954,6 +983,7 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     const int shift = shift_of((int)n[6]);
     if (!shared_sizes(B, Hq, Hk, D) || width < 1 || pages < 1) return -100;
     if (shift < 0) return -101;
+    if ((int64_t)B * width > MOST_KEYS >> shift) return -102;
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)plan | (uintptr_t)scratch) % 16 != 0) return -103;
     for (int i = 0; i < 8; ++i)
         if (sizes[i] % 8 != 0) return -103;

@@ -155,6 +155,8 @@ def test_tables_refused():
 
 @gpu
 def test_tables_refused_on_the_gpu():
+    with pytest.raises(ValueError, match="2 GiB"):
+        ops.KVPages([(torch.empty(1, 2 ** 27, 16, device="cuda", dtype=torch.uint8), None)])
     with pytest.raises(ValueError, match="16 bytes"):
         ops.KVPages([(torch.zeros(4, 8, 1, 6, dtype=torch.bfloat16, device="cuda"), None)])
     with pytest.raises(ValueError, match="cuda"):

@@ -203,6 +203,24 @@ def test_infinite_and_nan_values_stay_in_their_rows():
 
 
 @gpu
+@pytest.mark.parametrize("Hq,Hk", [(8, 2), (32, 2), (32, 1), (96, 1)])        # 4, 16, 32 and 96 columns a row
+@pytest.mark.parametrize("rows", [1, 3])
+def test_an_infinite_last_value(Hq, Hk, rows):
+    """Keys behind a chunk's last weigh nothing, whatever it holds."""
+    c = _case([(0, 3, 96 + 9 * i + 1) for i in range(rows)], Hq, Hk, seed=12)
+    table = c["block_table"]
+    for page, at in [(int(table[0, 3]), 0), (int(table[0, 2]), 31)]:          # row 0's last; all rows' last shared
+        c["v_cache"][page, at, :, 5] = float("inf")
+        c["v_cache"][page, at, :, 6] = float("-inf")
+        got = ops.attention_decode_shared(**c)
+        finite = torch.ones(128, dtype=torch.bool, device=got.device)
+        finite[5:7] = False
+        assert (got[0, :, 5] == float("inf")).all() and (got[0, :, 6] == float("-inf")).all()
+        assert torch.isfinite(got[..., finite]).all()
+    assert (got[:, :, 5] == float("inf")).all() and (got[:, :, 6] == float("-inf")).all()
+
+
+@gpu
 def test_large_scores():
     c = _case(GROUPS["ragged"], seed=11)
     c["q"] = c["q"] * 60
@@ -409,6 +427,8 @@ def test_random_batches():
     (lambda c: c.update(q=torch.empty(4 * 8 * 128 + 4, dtype=torch.bfloat16, device=DEVICE)[4:].view(4, 8, 128)),
      "16 bytes"),
     (lambda c: c.update(v_cache=c["v_cache"].cpu()), "one device"),
+    (lambda c: c.update(block_table=torch.zeros(4, 2 ** 18, dtype=torch.int32, device=DEVICE),
+                        **{x: c[x][:1, :1].expand(1, 2 ** 16, 8 // 4, 128) for x in ("k_cache", "v_cache")}), "2.35 tokens"),
 ])
 def test_refused(change, what):
     c = _case(GROUPS["ragged"], seed=20)
@@ -486,7 +506,7 @@ def test_entries_check_what_they_are_given():
     call = lambda n, q=16, scratch=16: lib.oa_attention_decode_shared(  # noqa: E731
         None, q, 16, 16, 16, None, None, None, 16, scratch, 16, (ctypes.c_int64 * 17)(*n), 0.1)
     for at, value, rc in [(9, 0, -100), (9, -1, -100), (13, 0, -100), (14, 0, -100), (14, 2 ** 31, -100),
-                          (15, 24, -101), (15, 0, -101), (0, 4092, -103), (4, 4, -103), (3, 2 ** 23, -105),
+                          (15, 24, -101), (15, 0, -101), (13, 2 ** 29, -102), (15, 2 ** 30, -102), (0, 4092, -103), (4, 4, -103), (3, 2 ** 23, -105),
                           (6, -8, -105)]:
         n = list(good)
         n[at] = value
@@ -495,6 +515,7 @@ def test_entries_check_what_they_are_given():
     assert lib.oa_shared_plan(None, 16, 16, 16, 8, 4, 32, 8, 128, 9, 32) == -103
     assert lib.oa_shared_plan(None, 16, 16, 16, 16, 4, 32, 8, 128, 0, 32) == -100
     assert lib.oa_shared_plan(None, 16, 16, 16, 16, 4, 32, 8, 128, 9, 33) == -101
+    assert lib.oa_shared_plan(None, 16, 16, 16, 16, 4, 32, 8, 128, 2 ** 29, 32) == -102
     bases = (ctypes.c_uint64 * 1)(4096)
     copy = lambda b, step, row, block, pages, c: lib.oa_kv_pages_copy(  # noqa: E731
         None, b, 1, step, row, block, pages, (ctypes.c_int * 3)(*c), 1)
