@@ -306,7 +306,7 @@ class LLMEngine:
         self._next_id = 1
         self._prefer_decode = False
         self.perf = get_perf_stats()
-        # decode graphs by (bucket, whether common blocks are read once); of hybrid models by bucket
+        # decode graphs by bucket, and those that read common blocks once
         self._graphs: Dict[int, Tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
         self._shared_graphs: Dict[int, Tuple[torch.cuda.CUDAGraph, torch.Tensor]] = {}
         pin = self.device == "cuda"
@@ -360,6 +360,12 @@ class LLMEngine:
         self._h_groups = torch.zeros(2, self.max_batch, dtype=torch.int32, pin_memory=pin)
         self._d_groups = torch.zeros(2, self.max_batch, dtype=torch.int32, device=dev)
         hq_local = self.spec.num_heads // self.tp
+        if self.shared_prefix and dev == "cuda":
+            # what the kernels of shared blocks do not take is refused here, not in a step
+            if self.dtype != torch.bfloat16:
+                raise ValueError(f"shared_prefix takes bfloat16 models, not {self.dtype}")
+            ops.shared_decode_plan(self._d_groups[0], *self._d_groups, (hq_local, hk_local),
+                                   self.spec.head_dim, self.max_blocks_per_seq, self.block_size)
         G = hq_local // hk_local if hk_local else 1
         # split count is frozen into the captured graph: size it for typical
         # agent sequence lengths (~1-2k), not max_seq — 64 splits of an 1.1k
@@ -460,7 +466,8 @@ class LLMEngine:
         self._next_id += 1
         req = Request(rid, list(prompt_ids), params)
         req.truncated_prompt_tokens = truncated
-        req.fork_of = None if self.hybrid else fork_of
+        # an earlier one: requests that wait for each other would wait for good
+        req.fork_of = fork_of if fork_of in self.requests and not self.hybrid else None
         if params.grammar is not None:
             req.grammar_state = GrammarState(
                 self.tokenizer, params.grammar, self.spec.vocab_size,
@@ -598,6 +605,9 @@ class LLMEngine:
             self.waiting.pop(at)
             req.fork_of = None
             if source is not None:
+                if any(dst in source.seq.blocks for _, dst, _ in copies):
+                    self.kv.copy_blocks(*zip(*copies))       # a fork of this step's own fork
+                    copies = []
                 req.seq, copy = source.seq.fork(len(req.prompt_ids))
                 copies += [copy] if copy else []
                 req.prefill_done = len(req.prompt_ids)

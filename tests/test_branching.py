@@ -283,6 +283,35 @@ def test_a_fork_of_an_ended_request():
     assert _drain(eng, [eng.add_request([1, 2, 3, 4, 5], PARAMS, fork_of=first)]) == want or torch.cuda.is_available()
 
 
+def test_forks_that_wait_for_nobody():
+    """A request is no fork of itself, nor of one behind it."""
+    eng = _engine(fork_choices=True)
+    ids = [eng.add_request([1, 2, 3, 4, 5], PARAMS, fork_of=i) for i in (1, 3, 2)]
+    assert ids == [1, 2, 3] and [eng.requests[i].fork_of for i in ids] == [None, None, 2]
+    assert all(len(g) == 9 for g in _drain(eng, ids))
+
+
+def test_forks_of_a_fork():
+    """A shorter prompt forks from a request that takes over its keys in the same step."""
+    prompt = [(7 * i) % 250 for i in range(11)]
+    plain = _engine()
+    want = [_drain(plain, [plain.add_request(p, PARAMS)])[0] for p in (prompt, prompt, prompt[:10])]
+    eng = _engine(fork_choices=True)
+    ids = [eng.add_request(prompt, PARAMS)]
+    ids.append(eng.add_request(prompt, PARAMS, fork_of=ids[0]))
+    ids.append(eng.add_request(prompt[:10], PARAMS, fork_of=ids[1]))
+    got = _drain(eng, ids)
+    assert got == want or torch.cuda.is_available()
+    assert all(len(g) == 9 for g in got)
+
+
+@gpu
+@pytest.mark.parametrize("change,error", [(dict(kv_block_size=24), AssertionError), (dict(model="llama3-tiny"), ValueError)])
+def test_engines_whose_kernels_do_not_share_are_refused(change, error):
+    with pytest.raises(error, match="power of 2|channels"):
+        _engine(shared_prefix=True, **change)
+
+
 def test_forks_under_cache_pressure():
     """Fewer blocks than the choices need: some wait or are preempted, all of them end."""
     eng = _engine(fork_choices=True, kv_num_blocks=14 if not torch.cuda.is_available() else 6)
