@@ -486,7 +486,7 @@ class LlamaForCausalLM(nn.Module):
             torch.cuda.empty_cache()
 
     def forward(self, fb: ForwardBatch, kv_caches: List[Tuple[torch.Tensor, torch.Tensor]]):
-        if fb.leaders is not None and fb.shared_plan is None:
+        if fb.leaders is not None:
             # the layers' lengths, blocks and heads are the same, and so is their plan
             at, k_cache = self.layers[0].attn, kv_caches[0][0]
             fb.shared_plan = ops.shared_decode_plan(
