@@ -1281,7 +1281,10 @@ class LLMEngine:
             if pad_to > B:
                 staged[B:pad_to] = staged[0]
         if shared:
-            self._h_rows[3][B:pad_to] = 0     # copies of row 0 read no keys
+            # here copies of row 0 read no keys, so that from the second layer on they are
+            # no copies: they are written nowhere
+            self._h_rows[2][B:pad_to] = -1
+            self._h_rows[3][B:pad_to] = 0
         used = self.max_batch * 5 + pad_to * self.max_blocks_per_seq
         self._d_step[:used].copy_(self._h_step[:used], non_blocking=True)
 

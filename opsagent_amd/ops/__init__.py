@@ -1484,6 +1484,7 @@ def rope_kv_fused(
     slot_mapping: torch.Tensor,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Fused RoPE(q,k in place) + paged KV write of k,v. Returns (q, k, v).
+    A row whose slot is negative is rotated and written nowhere.
 
     q/k/v may be head-slices of ONE fused [T, (Hq+2Hk)*D] qkv buffer sharing
     a token stride — no .contiguous() copies (those cost ~5.8 ms per 736-token
@@ -1491,7 +1492,8 @@ def rope_kv_fused(
     strides across q/k/v."""
     if not _is_gpu(q):
         q2, k2 = torch_ref.rope_apply(q, k, cos, sin, positions)
-        torch_ref.kv_cache_write(k_cache, v_cache, k2, v, slot_mapping.long())
+        kept = slot_mapping >= 0
+        torch_ref.kv_cache_write(k_cache, v_cache, k2[kept], v[kept], slot_mapping[kept].long())
         return q2, k2, v
     T, Hq, D = q.shape
     Hk = k.shape[1]

@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(
     uint32_t* __restrict__ vc,
     const float* __restrict__ cs, const float* __restrict__ sn,
     const int* __restrict__ positions,  // [T]
-    const int* __restrict__ slots,      // [T]
+    const int* __restrict__ slots,      // [T]; negative: a row that the cache does not take
     int T, int Hq, int Hk, int d2 /* D/2 */,
     int qts2, int kts2, int vts2 /* per-tensor token strides in words */,
     PLANES... planes) {
@@ -88,8 +88,9 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(
             ow2.y = pack_bf16x2(o2[2], o2[3]);
             *reinterpret_cast<uint2*>(row + dblk / 2) = ow1;
             *reinterpret_cast<uint2*>(row + (d2 + dblk) / 2) = ow2;
-            if (is_k) {
-                uint32_t* crow = kc + ((size_t)slots[it] * Hk + (h - Hq)) * d2;
+            const int slot = slots[it];
+            if (is_k && slot >= 0) {
+                uint32_t* crow = kc + ((size_t)slot * Hk + (h - Hq)) * d2;
                 *reinterpret_cast<uint2*>(crow + dblk / 2) = ow1;
                 *reinterpret_cast<uint2*>(crow + (d2 + dblk) / 2) = ow2;
             }
@@ -109,7 +110,8 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(
             } else {
                 val = *row;
             }
-            *reinterpret_cast<uint4*>(vc + ((size_t)slots[it] * Hk + h) * d2 + w4) = val;
+            const int slot = slots[it];
+            if (slot >= 0) *reinterpret_cast<uint4*>(vc + ((size_t)slot * Hk + h) * d2 + w4) = val;
         }
     }
 }
