@@ -17,10 +17,10 @@ cached (refcount 0) in LRU order and are evicted on allocation pressure.
 from __future__ import annotations
 
 import collections
-import functools
 import itertools
 from typing import Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from opsagent_amd import ops
@@ -320,44 +320,55 @@ def shared_prefixes(
             same += 1
         common.append(same)
 
-    # A group reads its blocks once, and each of its rows less by as many. Runs of rows with blocks in
-    # common are a tree; a run is a group or not, and rows go to the nearest group around them.
-    @functools.lru_cache(maxsize=None)
-    def best(lo: int, hi: int, around: int) -> Tuple[int, bool]:
-        """Blocks that rows lo..hi read less in a group of `around` blocks, or in better ones within
-        it; whether the run is a group of its own."""
-        if hi - lo == 1:
-            return around, False
-        least, parts = cut(lo, hi)
-        rest = sum(best(*p, around)[0] for p in parts)
-        own = sum(best(*p, least)[0] for p in parts) - least if least > around else rest
-        return (own, True) if own > rest else (rest, False)
+    # Runs of rows with blocks in common are a tree, run 0 all rows. Of each run: blocks in common,
+    # the run around it, rows that are in no run within it; and the runs, the inner ones first.
+    least, outer, own_rows = [0], [-1], [[]]
+    inner_first, under = [], [0]
 
-    @functools.lru_cache(maxsize=None)
-    def cut(lo: int, hi: int) -> Tuple[int, List[Tuple[int, int]]]:
-        least = min(common[lo : hi - 1])
-        edges = [lo] + [i + 1 for i in range(lo, hi - 1) if common[i] == least] + [hi]
-        return least, list(zip(edges, edges[1:]))
+    def begin(blocks: int) -> None:
+        under.append(len(least))
+        least.append(blocks)
+        outer.append(-1)
+        own_rows.append([])
 
-    # (run, blocks of the group around it, its rows); runs of 256 rows bound the depth
+    for b, ahead in zip(order, [*common, 0]):
+        if ahead > least[under[-1]]:
+            begin(ahead)
+        own_rows[under[-1]].append(b)
+        while least[under[-1]] > ahead:
+            run = under.pop()
+            if least[under[-1]] < ahead:
+                begin(ahead)            # a run that begins where this one did and goes on
+            outer[run] = under[-1]
+            inner_first.append(run)
+
+    # A group reads its blocks once, and each of its rows less by as many. A run is a group or not, and
+    # rows go to the nearest group around them. What a run saves hangs on the group around it: `around`
+    # has the blocks of the runs that may be that, from the outside, and `saves` what its rows save in
+    # a group of each, or in better ones within; the last is the run itself.
+    around, saves = {0: np.zeros(1, np.int64)}, {}
+    for run in reversed(inner_first):
+        around[run] = np.append(around[outer[run]], least[run])
+        saves[run] = len(own_rows[run]) * around[run]
+    saves[0] = np.zeros(1, np.int64)
+    for run in inner_first:
+        saves[outer[run]] += np.maximum(saves[run][:-1], saves[run][-1] - least[run])
+    # (blocks, rows) of the groups; of each run the place of its group in `around`, and the group's rows
     groups: List[Tuple[int, List[int]]] = []
-    work = [(lo, min(lo + 256, n), 0, None) for lo in range(0, n, 256)]
-    while work:
-        lo, hi, around, rows = work.pop()
-        if hi - lo == 1:
-            if rows is not None:
-                rows.append(order[lo])
-            continue
-        least, parts = cut(lo, hi)
-        if best(lo, hi, around)[1]:
-            around, rows = least, []
-            groups.append((least, rows))
-        work.extend((*part, around, rows) for part in parts)
+    place: Dict[int, Tuple[int, List[int]]] = {0: (0, [])}
+    for run in reversed(inner_first):
+        at, rows = place[outer[run]]
+        if saves[run][-1] - least[run] > saves[run][at]:
+            at, rows = len(around[run]) - 1, []
+            groups.append((least[run], rows))
+        rows += own_rows[run]
+        place[run] = at, rows
     for pages, rows in groups:
         if len(rows) > 1:
             saved += (len(rows) - 1) * pages
+            lead = min(rows)
             for b in rows:
-                leaders[b], shared[b] = min(rows), pages
+                leaders[b], shared[b] = lead, pages
     return leaders, shared, saved
 
 
