@@ -1232,16 +1232,19 @@ class LLMEngine:
         self.perf.record_metric("engine_decode_step_ms", (time.perf_counter() - t0) * 1000.0)
 
     def _find_shared(self, batch: List[Request]) -> bool:
-        """Whether the step reads blocks that its sequences have in common once; stages which."""
+        """Whether the step, whose block table is staged, reads blocks that its sequences have in
+        common once; stages which."""
+        weight = self.kv.block_size * (self.spec.num_kv_heads // self.tp)
         # sequences' common blocks change with the batch, and where one takes another's block
         key = (self.kv.switched, *(r.seq.serial for r in batch))
         if key != self._shared_key:
             self._shared_key = key
-            bs = self.kv.block_size
-            self._shared_groups = shared_prefixes(
-                [r.seq.blocks for r in batch], [len(r.seq.token_ids) // bs for r in batch])
+            full = [len(r.seq.token_ids) // self.kv.block_size for r in batch]
+            # all but the longest row's blocks are the most that can be saved
+            self._shared_groups = ([], [], 0) if (sum(full) - max(full)) * weight < SHARED_LEAST else (
+                shared_prefixes(self._h_rows[4].numpy(), full))
         leaders, pages, saved = self._shared_groups
-        if saved * self.kv.block_size * (self.spec.num_kv_heads // self.tp) < SHARED_LEAST:
+        if saved * weight < SHARED_LEAST:
             return False
         n = len(batch)
         groups = self._h_groups.numpy()
