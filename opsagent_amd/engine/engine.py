@@ -432,6 +432,8 @@ class LLMEngine:
         prompt. This one then waits for the other's prefill and takes over its keys (the model has
         to keep no recurrent state); it is prefilled by itself where the other has ended before."""
         given = prompt_ids, params
+        if not len(prompt_ids):
+            raise ValueError("a prompt has at least one token: there is nothing to go on from")
         if params.max_new_tokens >= self.max_seq_len:
             # a budget >= the context window would otherwise invert the
             # truncation slice below and empty the prompt
@@ -454,7 +456,7 @@ class LLMEngine:
             )
             self.perf.record_metric("engine_prompt_truncated_tokens", float(truncated))
             prompt_ids = prompt_ids[-keep:]
-        if len(prompt_ids) and not 0 <= min(prompt_ids) <= max(prompt_ids) < self.spec.vocab_size:
+        if not 0 <= min(prompt_ids) <= max(prompt_ids) < self.spec.vocab_size:
             # on the host: the device reads the embedding row of whatever id it is given
             raise ValueError(f"prompt token ids lie outside the model's vocabulary of "
                              f"{self.spec.vocab_size}")

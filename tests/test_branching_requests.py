@@ -1,0 +1,40 @@
+"""Requests that choices and forks are made of: those that an engine refuses, and those beside them."""
+
+import pytest
+import torch
+
+from opsagent_amd.engine.engine import LLMEngine, SamplingParams
+from opsagent_amd.engine.serving import EngineLoop
+
+PARAMS = SamplingParams(max_new_tokens=5, stop_on_eos=False)
+
+
+def _engine(**kw):
+    cfg = dict(model="llama3-tiny", max_batch_size=8, kv_block_size=4, max_seq_len=128, spec_decode=False)
+    if torch.cuda.is_available():
+        cfg.update(model="llama3-micro", kv_block_size=32, max_seq_len=1024, kv_num_blocks=300)
+    return LLMEngine({**cfg, **kw})
+
+
+@pytest.mark.parametrize("fork", [False, True])
+def test_an_empty_prompt_is_refused_by_itself(fork):
+    """It has no token to go on from; the requests beside it are answered."""
+    eng = _engine(fork_choices=fork)
+    with pytest.raises(ValueError, match="at least one token"):
+        eng.add_request([], PARAMS)
+    assert not eng.requests and not eng.waiting
+    loop = EngineLoop(eng)
+    try:
+        other = loop.submit([3, 4, 5], PARAMS)
+        empty = loop.submit_choices([], PARAMS, 3)
+        more = loop.submit_choices([5, 6, 7], PARAMS, 2)
+        for f in empty:
+            with pytest.raises(ValueError, match="at least one token"):
+                f.result(timeout=60)
+        assert all(len(f.result(timeout=60)[0]) == 5 for f in [other, *more])
+        tokens, last = loop.submit_stream([], PARAMS)
+        assert list(tokens) == []
+        with pytest.raises(ValueError, match="at least one token"):
+            last.result(timeout=60)
+    finally:
+        loop.shutdown()
