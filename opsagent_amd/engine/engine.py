@@ -213,6 +213,10 @@ class LLMEngine:
         self._shared_groups: Tuple[List[int], List[int], int] = ([], [], 0)
         # choices of one prompt take over the first one's keys instead of a prefill each
         self.fork_choices = bool(cfg.get("fork_choices", False)) and not self.hybrid
+        for option in ("shared_prefix", "fork_choices"):
+            if self.hybrid and cfg.get(option):
+                log.warning("%s is for models of the llama family: it does nothing for %s", option,
+                            self.spec.name)
         if self.spec.is_moe and (
             int(cfg.get("max_batch_size", 64)) * self.spec.moe_top_k > 2048
         ):

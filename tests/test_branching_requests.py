@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from opsagent_amd.engine import engine as engine_module
 from opsagent_amd.engine.engine import LLMEngine, SamplingParams
 from opsagent_amd.engine.serving import EngineLoop
 
@@ -38,3 +39,18 @@ def test_an_empty_prompt_is_refused_by_itself(fork):
             last.result(timeout=60)
     finally:
         loop.shutdown()
+
+
+def test_options_that_do_nothing_say_so(monkeypatch):
+    """Hybrid models share and fork nothing; an engine that is asked to warns, and answers."""
+    said = []
+    monkeypatch.setattr(engine_module.log, "warning", lambda text, *args: said.append(text % args))
+    hybrid = dict(model="povazen-tiny", kv_block_size=8, max_seq_len=64, kv_num_blocks=32, max_batch_size=4)
+    eng = LLMEngine({**hybrid, "fork_choices": True, "shared_prefix": True})
+    assert [t.split()[0] for t in said] == ["shared_prefix", "fork_choices"]
+    assert all("povazen-tiny" in t for t in said) and not eng.fork_choices and not eng.shared_prefix
+    assert len(eng.generate([1, 2, 3], PARAMS)[0]) == 5
+    said.clear()
+    LLMEngine(hybrid)
+    _engine(fork_choices=True, shared_prefix=True)
+    assert not said
