@@ -2023,7 +2023,11 @@ def attention_decode_shared(
     no keys. A group shares as many pages as all of its rows do, full ones only; what some of its
     rows share beyond that is read for each. ``plan``: of shared_decode_plan for these lengths and
     leaders; where it is None, a launch of up to 64 rows makes its own, and one of more is preceded by
-    one that does. No gradients."""
+    one that does. No gradients, of either mode."""
+    for t in (q, k_cache, v_cache):
+        if (t.requires_grad and torch.is_grad_enabled()) or (
+                forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError("shared decode attention has no gradients")
     if not _is_gpu(q):
         return torch_ref.attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders,
                                                  shared, scale)
@@ -2039,8 +2043,6 @@ def attention_decode_shared(
     at = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     if (at[0] | at[1] | at[2]) % 16:
         raise ValueError("q and caches begin at multiples of 16 bytes")
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise RuntimeError("shared decode attention has no gradients")
     if plan is not None and (plan.sizes != key or plan.ints.get_device() != device):
         raise ValueError(f"a plan of other sizes: {plan.sizes}, not {key}")
     if device != torch.cuda.current_device():
