@@ -5,6 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 from opsagent_amd import ops
+from test_shared_decode import _case, _check
 
 gpu = pytest.mark.gpu
 DEVICE = "cuda" if torch.cuda.is_available() else "cpu"
@@ -36,3 +37,75 @@ def test_gradients_of_either_mode_are_refused(name):
         with torch.no_grad(), pytest.raises(RuntimeError, match="gradients"):
             ops.attention_decode_shared(**dual)
         assert torch.equal(ops.attention_decode_shared(**c), want)
+
+
+def _long_batch(n):
+    """n rows, block 32: three groups that go through all of them, one led by the last row, strangers,
+    and rows without keys."""
+    rows = []
+    for b in range(n):
+        lead, pages = ((0, 3), (1, 1), (b, 0), (b, 0), (n - 1, 2), (0, 3), (0, 3))[b % 7]
+        rows.append((lead, pages, 0 if b % 7 == 3 else 32 * pages + 1 + (b * 7) % 40))
+    rows[0], rows[1], rows[n - 1] = (0, 3, 130), (1, 1, 33), (n - 1, 2, 64)
+    return rows
+
+
+@gpu
+@pytest.mark.parametrize("n,Hq,Hk,D,dtype", [
+    (256, 8, 2, 64, torch.bfloat16),
+    (257, 8, 2, 64, torch.bfloat16),
+    (300, 20, 1, 64, torch.float16),
+    (1024, 4, 4, 128, torch.bfloat16),
+    (1025, 6, 2, 64, torch.bfloat16),
+    (2047, 32, 8, 64, torch.float16),
+    (2048, 8, 2, 128, torch.bfloat16),
+    (2048, 128, 1, 64, torch.bfloat16),      # a tile is one row: the most partial results
+])
+def test_long_batches(n, Hq, Hk, D, dtype):
+    """Up to as many rows as there are: more than 256 are planned by a block of 1024 threads."""
+    c = _case(_long_batch(n), Hq, Hk, D, 32, dtype, seed=n)
+    got = ops.attention_decode_shared(**c)
+    _check(got, c)
+    plan = ops.shared_decode_plan(c["seq_lens"], c["leaders"], c["shared"], (Hq, Hk), D,
+                                  c["block_table"].shape[1], 32)
+    assert torch.equal(ops.attention_decode_shared(**c, plan=plan), got)
+
+
+@gpu
+def test_more_rows_than_a_plan_takes():
+    c = _case([(b, 0, 1) for b in range(2049)], 2, 1, 64, 32, seed=1)
+    with pytest.raises(ValueError, match="1 to 2048 rows"):
+        ops.attention_decode_shared(**c)
+    empty = {x: t[:0] if x not in ("k_cache", "v_cache") else t for x, t in c.items()}
+    with pytest.raises(ValueError, match="1 to 2048 rows"):
+        ops.attention_decode_shared(**empty)
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(30))
+def test_a_plan_made_by_the_launch_is_the_one_made_before(seed):
+    """Up to 64 rows are planned by each block for itself, or before: the same work, bit for bit."""
+    gen = torch.Generator().manual_seed(seed)
+    pick = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=gen))  # noqa: E731
+    n, leads, rows = (1, 2, 63, 64)[seed] if seed < 4 else pick(1, 64), [], []
+    span = (3, 60, 400, 1500)[pick(0, 3)]
+    for b in range(n):
+        kind = pick(0, 9)
+        if leads and kind < 6:
+            lead, pages = leads[pick(0, len(leads) - 1)]
+            rows.append((lead, pages, 16 * pages + pick(0, span)))
+        elif kind == 6:
+            rows.append((b, 0, 0))
+        else:
+            pages = pick(0, span // 16 + 1)
+            leads.append((b, pages))
+            rows.append((b, pages, 16 * pages + pick(1, span)))
+    group, Hk = pick(1, 20), pick(1, 5)
+    c = _case(rows, group * Hk, Hk, (64, 128)[seed % 2], 16, (torch.bfloat16, torch.float16)[seed // 2 % 2],
+              seed=200 + seed)
+    got = ops.attention_decode_shared(**c)
+    _check(got, c)
+    plan = ops.shared_decode_plan(c["seq_lens"], c["leaders"], c["shared"], (group * Hk, Hk), c["q"].shape[2],
+                                  c["block_table"].shape[1], 16)
+    assert torch.equal(ops.attention_decode_shared(**c, plan=plan), got)
+    assert torch.equal(ops.attention_decode_shared(**c), got)
