@@ -11,7 +11,9 @@
 // Sums, maxima and weight sums are float32. Weights enter the product with the values as 16-bit
 // numbers of the cache's type, as the matrix cores take them: off by half a step of each weight, which
 // averages out over the keys. Their sum is that of the rounded ones, so that what is divided by is what
-// was added up. The output is rounded to the same type.
+// was added up. float16 weights are taken 2^15 times as large, the largest power of 2 below its end:
+// those from 2^-29 of the largest on have all their bits, where 2^-14 would be the least. The output is
+// rounded to the same type.
 //
 // What bounds it (us; 32 heads on 8 and 64 on 8 of 128 channels, bfloat16): rows that share nothing, memory
 // (48 of up to 2000 tokens, 220 MB, 41: 5.4 TB/s); a few rows, latencies (a block's plan or its record 2
@@ -449,6 +451,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
     constexpr int PLANE = KEYS * ROW, STAGE = 2 * PLANE, NJ = KEYS / 16;
     constexpr int RPP = 1024 / ROW, PCS = 32 / RPP;          // rows of a transfer, transfers of 32 rows
     constexpr int COLS = CG * 32;
+    constexpr float LARGEST = F16 ? 15.0f : 0.0f;
     int lane = threadIdx.x & (WAVE - 1);
     asm volatile("" : "+v"(lane));           // places in LDS are worked out here, not kept from unit to unit
     const int col = lane & 15, g = lane >> 4;
@@ -573,6 +576,8 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
 #pragma unroll 1
         for (int at = (k1 - key) * ROW + from * 16; at < KEYS * ROW; at += 1024) *reinterpret_cast<uint4*>(vt + at) = uint4{0, 0, 0, 0};
     };
+    // the largest weight is 2^LARGEST
+    auto top_of = [&](float mx) { return mx * scale - LARGEST; };
     auto weights = [&](int key, char* vt) {
         if (key + KEYS > k1) {
             asm volatile("" : : : "memory");                 // a branch: every other step goes without
@@ -602,7 +607,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[m][d][r] *= keep;
             }
-            const float base = mx[m] == -INFINITY ? 0.0f : mx[m] * scale;
+            const float base = mx[m] == -INFINITY ? 0.0f : top_of(mx[m]);
 #pragma unroll
             for (int i = 0; i < NJ * 4; ++i)
                 sc[m][i >> 2][i & 3] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][i >> 2][i & 3], scale, -base));
@@ -720,7 +725,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
             for (int d = 0; d < ND; ++d) *reinterpret_cast<sh_f4*>(a.o_part + to * D + d * 16 + g * 4) = o[m][d];
             if (g == 0)
                 *reinterpret_cast<float2*>(a.ml_part + to * 2) =
-                    float2{mx[m] == -INFINITY ? -INFINITY : mx[m] * scale, sum[m][0]};
+                    float2{mx[m] == -INFINITY ? -INFINITY : top_of(mx[m]), sum[m][0]};
         }
         return;
     }
@@ -735,7 +740,7 @@ __device__ __forceinline__ void shared_unit(const SharedArgs& a, const SharedUni
         if (c >= columns) continue;
         if (g == 0)
             *reinterpret_cast<float2*>(stats + (kg * COLS + c) * 2) =
-                float2{mx[m] == -INFINITY ? -INFINITY : mx[m] * scale, sum[m][0]};
+                float2{mx[m] == -INFINITY ? -INFINITY : top_of(mx[m]), sum[m][0]};
 #pragma unroll
         for (int d = 0; d < ND; ++d)
             *reinterpret_cast<sh_f4*>(merge + (kg * COLS + c) * PITCH + d * 16 + g * 4) = o[m][d];

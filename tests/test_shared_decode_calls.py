@@ -109,3 +109,29 @@ def test_a_plan_made_by_the_launch_is_the_one_made_before(seed):
                                   c["block_table"].shape[1], 16)
     assert torch.equal(ops.attention_decode_shared(**c, plan=plan), got)
     assert torch.equal(ops.attention_decode_shared(**c), got)
+
+
+@gpu
+@pytest.mark.parametrize("columns", [4, 24, 48, 96])         # as the waves share keys and columns
+@pytest.mark.parametrize("shared", [False, True])
+def test_many_small_float16_weights(columns, shared):
+    """One key has nearly all of the weight, and what the others have in sum is not lost: weights down
+    to 2^-29 of the largest are rounded by half a step 2^-11 of each, like any other, and the output by as
+    much. float32 scores and exponentials are off by 2^-12 of what they weigh, as in other tests."""
+    n, D, rows = 2 ** 15, 64, 2 if shared else 1
+    heads = columns // rows
+    q = torch.zeros(rows, heads, D, dtype=torch.float16, device=DEVICE)
+    q[..., 0] = 4.0
+    k = torch.zeros(n // 64, 64, 1, D, dtype=torch.float16, device=DEVICE)
+    k[0, 0, 0, 0] = 4.5                                     # the others have 2^-25.97 of its weight
+    v = torch.zeros_like(k)
+    v[..., 1] = 1.0
+    v[0, 0, 0, 1] = 0.0
+    table = torch.arange(n // 64, dtype=torch.int32, device=DEVICE).expand(rows, -1).contiguous()
+    i32 = lambda x: torch.full((rows,), x, dtype=torch.int32, device=DEVICE)  # noqa: E731
+    got = ops.attention_decode_shared(q, k, v, table, i32(n), i32(0), i32(n // 64), scale=1.0)
+    small = torch.tensor(-18.0, dtype=torch.float64).exp()
+    want = float((n - 1) * small / (1 + (n - 1) * small))
+    h = 2.0 ** -11
+    assert want > 2.0 ** -11 and (got[..., 1].double() - want).abs().max() <= (2 * h + h * h + 2.0 ** -12) * want
+    assert torch.count_nonzero(got[..., 2:]) == 0
