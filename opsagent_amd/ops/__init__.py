@@ -2024,10 +2024,10 @@ def attention_decode_shared(
     rows share beyond that is read for each. ``plan``: of shared_decode_plan for these lengths and
     leaders; where it is None, a launch of up to 64 rows makes its own, and one of more is preceded by
     one that does. No gradients, of either mode."""
-    for t in (q, k_cache, v_cache):
-        if (t.requires_grad and torch.is_grad_enabled()) or (
-                forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
-            raise RuntimeError("shared decode attention has no gradients")
+    if (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)) or (
+            forward_ad._current_level >= 0
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k_cache, v_cache))):
+        raise RuntimeError("shared decode attention has no gradients")
     if not _is_gpu(q):
         return torch_ref.attention_decode_shared(q, k_cache, v_cache, block_table, seq_lens, leaders,
                                                  shared, scale)
