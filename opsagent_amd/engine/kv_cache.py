@@ -102,7 +102,8 @@ class PagedKVCache:
         """Keys and values of blocks src to blocks dst in all layers, or of their first tokens."""
         if len(src):
             if self._pages is None:
-                self._pages = ops.KVPages(self.layers)
+                self._pages = ops.KVPages([(k, v) if k is None else (k[: self.num_blocks], v[: self.num_blocks])
+                                           for k, v in self.layers])
             ops.kv_cache_copy(self._pages, src, dst, tokens)
 
     def drop_cached(self, keep: int = 0) -> int:
@@ -144,8 +145,10 @@ class PagedKVCache:
 
     def shrink(self, num_blocks: int, sequences: Sequence["SequenceState"]) -> None:
         """Gives memory back: the pool becomes its first `num_blocks`, compacted, cached blocks that
-        find no room dropped. The layers' tensors are new ones. Raises BlockAllocatorError where
-        sequences hold more blocks than that."""
+        find no room dropped. Layers' tensors that are longer become new ones. Raises
+        BlockAllocatorError where sequences hold more blocks than that. A layer that the device has
+        no memory to shorten stays as it is, and so do those behind it, while the error goes on to the
+        caller: the pool is sound, and can be shrunk again."""
         if not 0 < num_blocks <= self.num_blocks:
             raise ValueError(f"a pool of {self.num_blocks} blocks does not shrink to {num_blocks}")
         live = sum(1 for r in self._ref if r)
@@ -153,20 +156,20 @@ class PagedKVCache:
             raise BlockAllocatorError(f"{live} blocks are in use, more than {num_blocks}")
         self.drop_cached(num_blocks - live)
         self.compact(sequences)
-        self._pages = None
-        for i, (k, v) in enumerate(self.layers):
-            if k is None:
-                continue
-            # layer by layer: the peak is one layer more than the pool
-            self.layers[i] = (None, None)
-            prefix = v.data_ptr() == k.data_ptr()
-            vdim, keys = v.shape[-1], k[:num_blocks].clone()
-            values = keys[..., :vdim] if prefix else v[:num_blocks].clone()
-            del k, v
-            self.layers[i] = (keys, values)
+        # before the tensors: nobody names a block that one of them may lack
         del self._ref[num_blocks:], self._block_to_hash[num_blocks:], self._block_tokens[num_blocks:]
         self._free = collections.deque(b for b in self._free if b < num_blocks)
         self.num_blocks = num_blocks
+        self._pages = None
+        for i, (k, v) in enumerate(self.layers):
+            if k is None or k.shape[0] == num_blocks:
+                continue
+            # layer by layer: the peak is one layer more than the pool
+            prefix = v.data_ptr() == k.data_ptr()
+            vdim, keys = v.shape[-1], k[:num_blocks].clone()
+            values = keys[..., :vdim] if prefix else v[:num_blocks].clone()
+            self.layers[i] = (keys, values)
+            del k, v, keys, values
 
     # -- low-level allocator ----------------------------------------------
     def num_free(self) -> int:
