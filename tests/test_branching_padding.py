@@ -62,7 +62,7 @@ def _cached_rows(rows, shared, padded, steps=7):
     return out
 
 
-@pytest.mark.parametrize("rows", [3, 5, 7])
+@pytest.mark.parametrize("rows", [3, 5, 7, *(pytest.param(n, marks=gpu, id=f"{n}-captured") for n in (3, 5, 7))])
 def test_padding_rows_of_shared_steps_write_no_cache(rows, monkeypatch):
     """Rows that pad a shared step have no keys to attend to: what they compute is nobody's. The
     sequences' keys and values are those of a step without padding, and of one that shares nothing:
@@ -88,7 +88,8 @@ def _rotation_inputs(T, Hq, Hk, D, dtype):
 
 
 @pytest.mark.parametrize("T", [1, 4, 9])
-@pytest.mark.parametrize("parts", [False, pytest.param(True, marks=gpu)])
+@pytest.mark.parametrize("parts", [False, pytest.param(False, marks=gpu, id="gpu"),
+                                   pytest.param(True, marks=gpu, id="parts")])
 def test_rows_without_a_slot_are_written_nowhere(T, parts):
     Hq, Hk, D = 4, 2, 64
     c = _rotation_inputs(T, Hq, Hk, D, torch.bfloat16 if torch.cuda.is_available() else torch.float32)
