@@ -23,6 +23,7 @@ Architecture:
 from __future__ import annotations
 
 import dataclasses
+import threading
 import time
 from typing import Dict, List, Optional, Tuple
 
@@ -234,7 +235,7 @@ class LLMEngine:
         # request_bcast off, every rank must feed an identical request stream
         # itself (lockstep harness — debugging only).
         self.request_bcast = bool(cfg.get("request_bcast", True)) and self.tp > 1
-        self._bcast_pending: List[tuple] = []
+        self._bcast_pending: List[tuple] = []      # ("add", ids, params, fork_of) or ("shrink", blocks)
         self._bcast_flag: Optional[torch.Tensor] = None
         if self.request_bcast:
             import torch.distributed as dist
@@ -308,6 +309,7 @@ class LLMEngine:
         self.waiting: List[Request] = []
         self.running: List[Request] = []
         self._next_id = 1
+        self.stepping_thread: Optional[int] = None      # of a loop that runs the steps, while it does
         self._prefer_decode = False
         self.perf = get_perf_stats()
         # decode graphs by bucket, and those that read common blocks once
@@ -467,7 +469,7 @@ class LLMEngine:
         if self.request_bcast and self.tp_rank == 0:
             # record the PRE-normalization arguments; followers re-run this
             # exact function, so clamping/truncation replays identically
-            self._bcast_pending.append((list(given[0]), _params_to_wire(given[1]), fork_of))
+            self._bcast_pending.append(("add", list(given[0]), _params_to_wire(given[1]), fork_of))
         rid = self._next_id
         self._next_id += 1
         req = Request(rid, list(prompt_ids), params)
@@ -571,8 +573,12 @@ class LLMEngine:
             if n > 0:
                 buf: List[Optional[list]] = [None]
                 dist.broadcast_object_list(buf, src=0)
-                for ids, wire, fork_of in buf[0]:
-                    self.add_request(ids, _params_from_wire(wire), fork_of)
+                for kind, *what in buf[0]:
+                    if kind == "shrink":
+                        self.shrink_cache(*what)
+                    else:
+                        ids, wire, fork_of = what
+                        self.add_request(ids, _params_from_wire(wire), fork_of)
             self.step()
             # no consumer on followers: reap finished requests immediately
             done = [rid for rid, r in self.requests.items() if r.finished]
@@ -1262,8 +1268,15 @@ class LLMEngine:
 
     def shrink_cache(self, num_blocks: int) -> None:
         """Gives memory of the key/value pool back, between steps: running sequences keep their
-        keys, the prefix cache what finds room. Decode graphs are captured again. At TP>1 every
-        rank calls it before the same step."""
+        keys, the prefix cache what finds room. Decode graphs are captured again. Refused while the
+        thread of an EngineLoop runs the steps: EngineLoop.shrink_cache is for that. At TP>1 rank 0
+        calls it, and the others follow before their next step; without request_bcast every rank
+        calls it before the same step."""
+        if self.stepping_thread not in (None, threading.get_ident()):
+            raise RuntimeError("another thread runs the engine's steps: EngineLoop.shrink_cache shrinks between them")
+        self.kv.check_shrink(num_blocks)          # raises before anything has changed, on any rank
+        if self.request_bcast and self.tp_rank == 0:
+            self._bcast_pending.append(("shrink", num_blocks))
         if self.device == "cuda":
             torch.cuda.synchronize()
         self._graphs.clear()

@@ -143,18 +143,22 @@ class PagedKVCache:
             seq.blocks = [to.get(b, b) for b in seq.blocks]
         return n
 
+    def check_shrink(self, num_blocks: int) -> int:
+        """Blocks in use. Raises what `shrink` does, where it would."""
+        if not 0 < num_blocks <= self.num_blocks:
+            raise ValueError(f"a pool of {self.num_blocks} blocks does not shrink to {num_blocks}")
+        live = sum(1 for r in self._ref if r)
+        if live > num_blocks:
+            raise BlockAllocatorError(f"{live} blocks are in use, more than {num_blocks}")
+        return live
+
     def shrink(self, num_blocks: int, sequences: Sequence["SequenceState"]) -> None:
         """Gives memory back: the pool becomes its first `num_blocks`, compacted, cached blocks that
         find no room dropped. Layers' tensors that are longer become new ones. Raises
         BlockAllocatorError where sequences hold more blocks than that. A layer that the device has
         no memory to shorten stays as it is, and so do those behind it, while the error goes on to the
         caller: the pool is sound, and can be shrunk again."""
-        if not 0 < num_blocks <= self.num_blocks:
-            raise ValueError(f"a pool of {self.num_blocks} blocks does not shrink to {num_blocks}")
-        live = sum(1 for r in self._ref if r)
-        if live > num_blocks:
-            raise BlockAllocatorError(f"{live} blocks are in use, more than {num_blocks}")
-        self.drop_cached(num_blocks - live)
+        self.drop_cached(num_blocks - self.check_shrink(num_blocks))
         self.compact(sequences)
         # before the tensors: nobody names a block that one of them may lack
         del self._ref[num_blocks:], self._block_to_hash[num_blocks:], self._block_tokens[num_blocks:]

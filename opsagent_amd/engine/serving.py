@@ -13,6 +13,7 @@ from __future__ import annotations
 import queue
 import threading
 from concurrent.futures import Future
+from concurrent.futures import TimeoutError as FutureTimeout
 from typing import Dict, List, Optional
 
 from opsagent_amd.engine.engine import LLMEngine, SamplingParams
@@ -37,6 +38,7 @@ class EngineLoop:
         self._step_started: float = 0.0
         self._submit_q: "queue.Queue[Tuple[List[int], SamplingParams, Future]]" = queue.Queue()
         self._futures: Dict[int, Future] = {}
+        self._shrink_q: "queue.Queue[Tuple[int, Future]]" = queue.Queue()
         self._wake = threading.Event()
         self._stop = False
         self._stopped = threading.Event()
@@ -48,6 +50,7 @@ class EngineLoop:
             return
         self._thread = threading.Thread(target=self._run, name="engine-loop", daemon=True)
         self._thread.start()
+        engine.stepping_thread = self._thread.ident
         self._watchdog = threading.Thread(target=self._watch, name="engine-watchdog", daemon=True)
         self._watchdog.start()
 
@@ -115,6 +118,24 @@ class EngineLoop:
 
         return _iter(), fut
 
+    def shrink_cache(self, num_blocks: int) -> None:
+        """The engine's shrink_cache, from any thread: between two steps of the loop. Returns when the
+        pool has its new size, and raises what that raises."""
+        if self.is_follower:
+            raise RuntimeError("TP follower ranks shrink with rank 0 — call it there")
+        if threading.current_thread() is self._thread:
+            return self.engine.shrink_cache(num_blocks)       # a future's callback: between steps
+        done: Future = Future()
+        self._shrink_q.put((num_blocks, done))
+        self._wake.set()
+        while True:
+            alive = self._thread.is_alive()
+            try:
+                return done.result(timeout=0.2)
+            except FutureTimeout:
+                if not alive and not done.done():
+                    raise RuntimeError("the engine loop has ended") from None
+
     def shutdown(self) -> None:
         self._stop = True
         if self.is_follower:
@@ -150,9 +171,27 @@ class EngineLoop:
                 if tq is not None:
                     tq.put(None)
 
+    def _shrink(self) -> None:
+        while True:
+            try:
+                num_blocks, done = self._shrink_q.get_nowait()
+            except queue.Empty:
+                return
+            try:
+                done.set_result(self.engine.shrink_cache(num_blocks))
+            except Exception as e:  # noqa: BLE001 — the caller's
+                done.set_exception(e)
+
     def _run(self) -> None:
+        try:
+            self._steps()
+        finally:
+            self.engine.stepping_thread = None
+
+    def _steps(self) -> None:
         eng = self.engine
         while not self._stop:
+            self._shrink()
             self._drain_submissions()
             if not eng.running and not eng.waiting:
                 self._wake.wait(timeout=0.05)
