@@ -1938,6 +1938,8 @@ def _shared_table(B: int, width: int, block: int) -> None:
         raise ValueError(f"a table of {width} pages of {block} tokens, which is no power of 2")
     if B * width * block > 2 ** 35:
         raise ValueError(f"tables of more than 2^35 tokens in all: {B} rows of {width} pages of {block}")
+    if width * block > 2 ** 31 - 2 ** 20:
+        raise ValueError(f"a row of more than 2^31 - 2^20 tokens: {width} pages of {block}")
 
 
 def _int_rows(B: int, **rows: torch.Tensor) -> None:
@@ -2016,7 +2018,8 @@ def attention_decode_shared(
 ) -> torch.Tensor:
     """attention_decode_paged of a batch whose sequences begin with the same pages: those are read
     once for all of them. q [B, Hq, D]; caches [pages, block, Hk, D] of q's type (bfloat16, float16;
-    64 or 128 channels); block_table [B, width] int32; out [B, Hq, D], zeros for rows without keys.
+    64 or 128 channels); block_table [B, width] int32, with room for 2^31 - 2^20 tokens a row and 2^35 in
+    all; out [B, Hq, D], zeros for rows without keys.
 
     leaders, shared [B] int32: the first shared[b] pages of row b are those of row leaders[b]. A row
     that shares nothing leads itself; so does one whose leader is no row that leads itself, or has

@@ -69,6 +69,8 @@ constexpr int PLAN_ROWS = 2048;
 constexpr int TILE = 128;                          // columns that a block takes
 constexpr int SIZES = 8;                           // sizes of an item that are looked at
 constexpr int64_t MOST_KEYS = (int64_t)1 << 35;    // that tables have room for: sizes and 8 of them are 32 bits
+// that a row's table has room for: up to 513 chunks of a row's keys, rounded up to 128, end within 32 bits
+constexpr int64_t MOST_ROW = ((int64_t)1 << 31) - (1 << 20);
 
 struct PlanSizes {
     int B, G, width, shift, tile, runs, max_units, max_slots;    // tile: members of TILE columns
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(THREADS) void shared_plan_kernel(const int* __restr
         place[ROWS], unit_of[ROWS];
     __shared__ uint32_t line[ROWS], total[NW], items_of[SIZES];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE, B = z.B;
-    const int most = (int)min((int64_t)z.width << z.shift, (int64_t)INT32_MAX - 4096);
+    const int most = z.width << z.shift;
     auto wave_total = [](int v) { return __builtin_amdgcn_readlane(wave_sums(v), WAVE - 1); };
     for (int b = tid; b < B; b += THREADS) {
         keys[b] = min(max(seq_lens[b], 0), most);
@@ -325,7 +327,7 @@ __device__ __forceinline__ void plan_item(const SharedArgs& a, int item, OwnPlan
     asm volatile("" : "+v"(lane));                           // nothing of this is kept meanwhile
     const int B = z.B;
     const bool in = lane < B;
-    const int most = (int)min((int64_t)z.width << z.shift, (int64_t)INT32_MAX - 4096);
+    const int most = z.width << z.shift;
     const int keys = in ? min(max(a.seq_lens[lane], 0), most) : 0;
     const int l = in ? a.leaders[lane] : lane, sh = in ? a.shared[lane] : 0;
     own.count[lane] = 0;
@@ -926,6 +928,10 @@ static bool shared_sizes(int B, int Hq, int Hk, int D) {
     return B >= 1 && B <= PLAN_ROWS && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Hq <= 4096 && Hq / Hk <= TILE && (D == 64 || D == 128);
 }
 
+static bool table_sizes(int B, int width, int shift) {
+    return (int64_t)B * width <= MOST_KEYS >> shift && width <= MOST_ROW >> shift;
+}
+
 // Blocks of a key head: two a CU. Units: items, of which there are at the most `runs` and one for each
 // tile of a group (B / tile and one more for each of B / 2 groups) beside as many of the line, and one
 // more a row. Slots: what an item of a tile leaves is a slot for each of its members, of which there
@@ -973,7 +979,7 @@ extern "C" int oa_shared_plan(void* stream, const void* seq_lens, const void* le
     if (!shared_sizes(B, Hq, Hk, D) || width < 1) return -100;
     const int shift = shift_of(block_size);
     if (shift < 0) return -101;
-    if ((int64_t)B * width > MOST_KEYS >> shift) return -102;
+    if (!table_sizes(B, width, shift)) return -102;
     if ((uintptr_t)plan % 16 != 0) return -103;
     return launch_plan((hipStream_t)stream, seq_lens, leaders, shared, plan, plan_sizes(B, Hq, Hk, width, shift));
 }
@@ -992,7 +998,7 @@ extern "C" int oa_attention_decode_shared(void* stream, const void* q, const voi
     const int shift = shift_of((int)n[6]);
     if (!shared_sizes(B, Hq, Hk, D) || width < 1 || pages < 1) return -100;
     if (shift < 0) return -101;
-    if ((int64_t)B * width > MOST_KEYS >> shift) return -102;
+    if (!table_sizes(B, width, shift)) return -102;
     if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)plan | (uintptr_t)scratch) % 16 != 0) return -103;
     for (int i = 0; i < 8; ++i)
         if (sizes[i] % 8 != 0) return -103;

@@ -1,5 +1,8 @@
 """Calls of shared decode attention beside those of a serving step: what is refused, long batches, plans."""
 
+import ctypes
+import os
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -135,3 +138,36 @@ def test_many_small_float16_weights(columns, shared):
     h = 2.0 ** -11
     assert want > 2.0 ** -11 and (got[..., 1].double() - want).abs().max() <= (2 * h + h * h + 2.0 ** -12) * want
     assert torch.count_nonzero(got[..., 2:]) == 0
+
+
+# -- the longest rows ----------------------------------------------------------------------------
+def _last_end(keys, blocks):
+    """Where the last of a group's chunks ends, as the plan works it out, before it is cut to `keys`."""
+    up = lambda a, b: -(-a // b)  # noqa: E731
+    sizes = up(keys, 64)
+    run = max(2, up(sizes + 1, blocks))
+    chunk = up(up(keys, up(sizes, run)), 128) * 128
+    return up(keys, chunk) * chunk
+
+
+def test_rows_whose_chunks_end_past_32_bits_are_refused():
+    """The last chunk of a row of nearly 2^31 tokens ends past them; a table may have room for 2^31 - 2^20."""
+    assert max(_last_end(2 ** 31 - 4096 - i, 512) for i in range(5000)) >= 2 ** 31
+    most = 2 ** 31 - 2 ** 20
+    assert max(_last_end(most - i, n) for i in range(3000) for n in (1, 2, 8, 64, 512)) < 2 ** 31
+    ops._shared_table(1, most // 2 ** 20, 2 ** 20)
+    for width, block in [(2 ** 11, 2 ** 20), (most // 16 + 1, 16), (most + 1, 1)]:
+        with pytest.raises(ValueError, match="a row of more than"):
+            ops._shared_table(1, width, block)
+    path = os.path.join(os.path.dirname(ops.__file__), "libopsagent_kernels.so")
+    if not os.path.exists(path):
+        pytest.skip("kernel library not built")
+    from opsagent_amd.ops import hip_lib
+
+    lib = ctypes.CDLL(path)
+    hip_lib._declare(lib)
+    for width, block in [(2 ** 11, 2 ** 20), (most // 16 + 1, 16), (most + 1, 1)]:
+        assert lib.oa_shared_plan(None, 16, 16, 16, 16, 1, 32, 8, 128, width, block) == -102
+        n = [4096, 128, 262144, 1024, 128, 262144, 1024, 128, 9, 1, 32, 8, 128, width, 50, block, 0]
+        assert lib.oa_attention_decode_shared(None, 16, 16, 16, 16, None, None, None, 16, 16, 16,
+                                              (ctypes.c_int64 * 17)(*n), 0.1) == -102
