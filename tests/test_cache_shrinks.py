@@ -90,6 +90,32 @@ def test_the_same_size_is_no_copy():
         cache.shrink(2, [seq])
 
 
+@pytest.mark.parametrize("shapes", SHAPES)
+@pytest.mark.parametrize("room,hits", [(0, {0: 0, 2: 0}), (1, {0: 0, 2: 0}), (2, {0: 0, 2: 8}), (3, {0: 4, 2: 8}),
+                                       (9, {0: 4, 2: 8})])
+def test_what_the_prefix_cache_finds_after_a_shrink(shapes, room, hits):
+    """Three blocks are cached: the first sequence's one, then the third's two. The oldest go first, so
+    that with room for one it is the third's second, which nothing reaches without its first."""
+    cache = _cache(shapes, blocks=24)
+    tokens = [[100 * i + j for j in range(4 + 3 * i)] for i in range(5)]
+    seqs = [_sequence(cache, t) for t in tokens]
+    before = {i: _rows(cache, seqs[i].blocks) for i in range(5)}
+    for i in (0, 2):
+        seqs[i].free()
+    live = [seqs[i] for i in (1, 3, 4)]
+    used = len({b for s in live for b in s.blocks})
+    cache.shrink(used + room, live)
+    assert cache.num_free() == room and all(s.blocks and max(s.blocks) < used + room for s in live)
+    for i in range(5):
+        found = SequenceState(cache, tokens[i] + [7])
+        reused = found.reuse_prefix()
+        assert reused == (hits[i] if i in hits else len(tokens[i]) // 4 * 4)
+        full = reused // 4
+        assert _same(_rows(cache, found.blocks), [t[:full] for t in before[i]])
+        found.free()
+    assert cache.num_free() == room
+
+
 # -- under a loop ----------------------------------------------------------------------------------
 PARAMS = SamplingParams(max_new_tokens=40, stop_on_eos=False)
 
