@@ -474,8 +474,11 @@ class LLMEngine:
         self._next_id += 1
         req = Request(rid, list(prompt_ids), params)
         req.truncated_prompt_tokens = truncated
-        # an earlier one: requests that wait for each other would wait for good
-        req.fork_of = fork_of if fork_of in self.requests and not self.hybrid else None
+        # an earlier one: requests that wait for each other would wait for good. Prompts are compared
+        # here and not in the steps that wait: a prompt only grows, when its request is preempted.
+        source = None if self.hybrid else self.requests.get(fork_of)
+        if source is not None and source.prompt_ids[: len(req.prompt_ids)] == req.prompt_ids:
+            req.fork_of = fork_of
         if params.grammar is not None:
             req.grammar_state = GrammarState(
                 self.tokenizer, params.grammar, self.spec.vocab_size,
@@ -688,10 +691,9 @@ class LLMEngine:
         """The request whose keys `req` takes over, and whether it has them yet. None: `req` has a
         prefill of its own."""
         source = None if req.fork_of is None else self.requests.get(req.fork_of)
-        n = len(req.prompt_ids)
-        if source is None or source.finished or source.prompt_ids[:n] != req.prompt_ids:
+        if source is None or source.finished:
             return None, True
-        return source, source.seq is not None and source.seq.num_cached >= n
+        return source, source.seq is not None and source.seq.num_cached >= len(req.prompt_ids)
 
     def _preempt(self, req: Request) -> None:
         """Out of KV blocks: return the request to the FRONT of the waiting

@@ -54,3 +54,34 @@ def test_options_that_do_nothing_say_so(monkeypatch):
     LLMEngine(hybrid)
     _engine(fork_choices=True, shared_prefix=True)
     assert not said
+
+
+def test_prompts_are_compared_once():
+    """A long prompt's choices wait for many steps of its prefill, and compare nothing meanwhile."""
+    eng = _engine(fork_choices=True, max_prefill_chunk=2)
+    prompt = [3, 4, 5, 6, 7, 8, 9, 10, 11]
+    compared = []
+
+    class Tokens(list):
+        def __getitem__(self, at):
+            if isinstance(at, slice) and at.start is None:
+                compared.append(at)
+            return list.__getitem__(self, at)
+
+    first = eng.add_request(prompt, PARAMS)
+    eng.requests[first].prompt_ids = Tokens(prompt)
+    same = [eng.add_request(prompt, PARAMS, fork_of=first) for _ in range(2)]
+    shorter = eng.add_request(prompt[:5], PARAMS, fork_of=first)
+    other = eng.add_request(prompt[:5] + [1], PARAMS, fork_of=first)
+    longer = eng.add_request(prompt + [1], PARAMS, fork_of=first)
+    assert [eng.requests[i].fork_of for i in (*same, shorter, other, longer)] == [first] * 3 + [None] * 2
+    assert len(compared) == 5
+    ids = [first, *same, shorter, other, longer]
+    for _ in range(100):
+        eng.step()
+        if all(eng.requests[i].finished for i in ids):
+            break
+    assert len(compared) == 5
+    out = {i: eng.requests[i].output_ids for i in ids}
+    assert all(len(t) == 5 for t in out.values()) and out[same[0]] == out[same[1]]
+    assert out[first] == out[same[0]] or torch.cuda.is_available()
