@@ -88,8 +88,8 @@ __global__ __launch_bounds__(256) void rope_kv_kernel(
             ow2.y = pack_bf16x2(o2[2], o2[3]);
             *reinterpret_cast<uint2*>(row + dblk / 2) = ow1;
             *reinterpret_cast<uint2*>(row + (d2 + dblk) / 2) = ow2;
-            const int slot = slots[it];
-            if (is_k && slot >= 0) {
+            const int slot = is_k ? slots[it] : -1;
+            if (slot >= 0) {
                 uint32_t* crow = kc + ((size_t)slot * Hk + (h - Hq)) * d2;
                 *reinterpret_cast<uint2*>(crow + dblk / 2) = ow1;
                 *reinterpret_cast<uint2*>(crow + (d2 + dblk) / 2) = ow2;
