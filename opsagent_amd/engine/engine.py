@@ -136,7 +136,10 @@ _BCAST_MARK = -2
 # A layer's rotation and attention, us, rows apart / common blocks once, 150 tokens behind them: 32
 # heads on 8, 8 rows behind 1024 tokens (57k) 15.4 / 15.7, behind 4096 (229k) 27.8 / 19.7, 32 behind
 # 512 (127k) 19.8 / 22.5, behind 1024 (254k) 26.6 / 23.7, behind 8192 114 / 31, 64 behind 8192 210 / 38;
-# 8 on 2, 16 behind 4096 (123k) 19.3 / 18.9, 32 behind 4096 (254k) 28.3 / 23.5.
+# 8 on 2, 16 behind 4096 (123k) 19.3 / 18.9, 32 behind 4096 (254k) 28.3 / 23.5. Nothing that was measured
+# above the line is slower. It does not count the query heads of a key head, and is too high for eight of
+# them: 64 on 8, 4 behind 4096 (98k) 24.2 / 19.4, 8 behind 2048 (115k) 25.7 / 19.3, 32 behind 512 (127k)
+# 27.2 / 23.3; a little for four: 32 on 8, 8 behind 2048 (115k) 19.6 / 16.7.
 SHARED_LEAST = 1 << 17
 
 

@@ -19,7 +19,8 @@
 // (48 of up to 2000 tokens, 220 MB, 41: 5.4 TB/s); a few rows, latencies (a block's plan or its record 2
 // to 3, first keys 2, a step 1, sums 1; the second launch 3); many rows behind one prefix, matrix and
 // vector instructions of steps of 128 columns, 2.2 us for two blocks of a CU and 64 keys (128 rows
-// behind 16400 tokens 116 in all, 0.6 PFLOP/s).
+// behind 16400 tokens 116 in all, 0.6 PFLOP/s: of 64 blocks of a key head 48 take 44 such steps each, 16 the
+// rows' own keys, which end sooner).
 //
 //   q            [B, Hq, D] 16-bit, rows and heads any multiple of 8 elements apart
 //   kc, vc       [pages, 2^shift, Hk, D], pages, tokens and heads any multiple of 8 elements apart
@@ -935,7 +936,8 @@ static bool table_sizes(int B, int width, int shift) {
 // Blocks of a key head: two a CU. Units: items, of which there are at the most `runs` and one for each
 // tile of a group (B / tile and one more for each of B / 2 groups) beside as many of the line, and one
 // more a row. Slots: what an item of a tile leaves is a slot for each of its members, of which there
-// are `tile` or B, and a row has one more of each kind than equal shares would make.
+// are `tile` or B, and a row has one more of each kind than equal shares would make. Many rows of many heads
+// on few take the most memory for them: 2048 of 128 on 1, of 128 channels, 0.6 GB.
 static PlanSizes plan_sizes(int B, int Hq, int Hk, int width, int shift) {
     PlanSizes z;
     z.B = B;
