@@ -27,7 +27,7 @@ static_assert(sizeof(PageTensors) + sizeof(PageCopies) + 32 <= 4096, "what a lau
 // thread. What is written is not kept: it is more than the next reader's share of a cache where it
 // takes time at all. us, by size: 96 pages of 64 KiB in 64 tensors (805 MB in and out) 128 (6.3 TB/s;
 // kept 135, tensors side by side 157, 64 bytes a thread 162), three copies of 16 pages' first tokens in
-// 160 tensors (291 MB) 66 (77, 78, 99), three of one in 64 4, with the launch. From one box to another,
+// 160 tensors (291 MB) 66 (77, 78, 99), three of one in 64 4, with the launch. From one card to another,
 // and with how much of the caches the last copy left, those of 16 pages take 47 to 82.
 __global__ __launch_bounds__(256) void kv_pages_copy_kernel(PageTensors tensors, PageCopies copies,
                                                             int64_t step, int row) {
